@@ -447,9 +447,143 @@ int sg_gather_rows(const void* const* src_dev, int32_t num_src, int64_t src_row_
                    int32_t num_index, void* out_dev, int64_t out_row_stride,
                    int32_t* status_dev, sg_stream_t stream);
 
+/* ------------------------------------------------------------------------
+ * (E) The cache in 4 bits.
+ *
+ * No reference counterpart (its caches are bf16).  A K or V row of D values is
+ * D/2 bytes of codes and D/32 bytes of scales, the microscaling format with
+ * e2m1 elements: element 2i is the low nibble of byte i, element 2i+1 the high
+ * one; a nibble is a sign bit over a magnitude of 0, 1/2, 1, 3/2, 2, 3, 4 or 6;
+ * scale byte j, of elements 32j .. 32j+31, stands for 2^(byte - 127), 255 for
+ * NaN.  Packing takes the least power of two of which the block's largest
+ * magnitude is at most 7 times, so that every element is off by at most half a
+ * step where it lies (bytes 1 to 252: a smaller block is rounded to multiples of
+ * 2^-127, a larger one saturates at 6 * 2^125), rounds to nearest, ties to the
+ * even code, and gives a block with an infinity or a NaN the scale 255 and codes
+ * 0.  Every value is a bf16 value.
+ * ---------------------------------------------------------------------- */
+
+/* sg_kv_commit into a 4-bit arena: the kept bf16 tree rows of every layer are
+ * packed and appended,
+ *   row (g, prefix_start_i + len_i + t) = packed(tree[l][row_offset_i + keep_i[t], g]),
+ * then len_i += keep_len_i.  Its conditions and status words are sg_kv_commit's;
+ * strides of codes and scales are in bytes. */
+typedef struct SgKvCommitMx4Args {
+  int32_t num_layers;
+  int32_t num_requests;
+  int32_t num_kv_heads;
+  int32_t head_dim;                /* multiple of 32 */
+  /* per-layer bases of the arena (device arrays of num_layers device pointers) */
+  void* const* k_code_layers_dev;
+  void* const* k_scale_layers_dev;
+  void* const* v_code_layers_dev;
+  void* const* v_scale_layers_dev;
+  int64_t code_head_stride, code_token_stride;    /* multiples of 4; bases 4-byte aligned */
+  int64_t scale_head_stride, scale_token_stride;
+  /* per-layer tree-row K/V bases [R, Hkv, D] bf16 (device arrays of pointers) */
+  const void* const* k_tree_layers_dev;
+  const void* const* v_tree_layers_dev;
+  int64_t tree_row_stride, tree_head_stride;
+  const int32_t* row_offset_dev;   /* [n+1] packed row range of request i */
+  const int32_t* keep_rows_dev;    /* [n, keep_stride] local rows; NULL: rows 0 .. keep_len-1 */
+  int32_t keep_stride;             /* most rows a request keeps */
+  const int32_t* keep_len_dev;     /* [n] */
+  const int64_t* prefix_start_dev; /* [n] slot_i * capacity */
+  int32_t* lengths_dev;            /* [n] cached length of request i; advanced in place */
+  int32_t capacity;
+  int32_t* status_dev;             /* optional [1]; SG_ERANGE or SG_EINVAL, never cleared */
+} SgKvCommitMx4Args;
+
+int sg_kv_commit_mx4(const SgKvCommitMx4Args* args, sg_stream_t stream);
+
+/* bf16 values of packed rows: out[o, t, :] from codes[o, t, :], scales[o, t, :]
+ * for o < outer, t < tokens.  Strides of codes (multiples of 4) and scales are in
+ * bytes, of out (multiples of 8) in elements. */
+int sg_kv_load_mx4(const void* codes_dev, int64_t code_outer_stride, int64_t code_token_stride,
+                   const void* scales_dev, int64_t scale_outer_stride,
+                   int64_t scale_token_stride, int32_t outer, int32_t tokens, int32_t head_dim,
+                   void* out_dev, int64_t out_outer_stride, int64_t out_token_stride,
+                   sg_stream_t stream);
+
+/* sg_tree_attn_fwd over a 4-bit prefix (the wave's own rows are bf16). */
+typedef struct SgTreeAttnMx4Args {
+  SgTreeAttnArgs attn;        /* k/v_cache_dev: codes, 16-byte aligned; the cache strides are
+                                 in bytes, multiples of 16.  Plans are sg_tree_attn_plan's */
+  const void* k_scale_dev;    /* scales [Hkv, tokens, D/32] */
+  const void* v_scale_dev;
+  int64_t scale_head_stride, scale_token_stride;  /* bytes */
+} SgTreeAttnMx4Args;
+
+int sg_tree_attn_mx4_fwd(const SgTreeAttnMx4Args* args, sg_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * (F) Projections in 8-bit floating point.
+ *
+ * No reference counterpart (its projections are the transformers modules').
+ * Values are e4m3 (the finite form: largest 448, no infinities) times fp32
+ * scales: activations have one for each row and 128 columns, made by the kernel
+ * that produces them,
+ *   m = max(max |x|, 2^-100), code = e4m3(x * (448 / m)), scale = m / 448,
+ * weights one for each 128 x 128 block.  Codes are [R, Kp], Kp = K rounded up to
+ * 128, columns K .. Kp-1 zero; scales are [Kp/128, scale_stride] with row r's at
+ * column r.  A block with an infinity or a NaN gives NaN codes or a NaN scale.
+ * ---------------------------------------------------------------------- */
+typedef struct SgFp8RowsOut {
+  void* codes_dev;               /* e4m3 [R, code_stride] */
+  int64_t code_stride;           /* >= Kp, a multiple of 16 */
+  float* scales_dev;             /* [Kp/128, scale_stride] */
+  int64_t scale_stride;          /* >= R */
+} SgFp8RowsOut;
+
+/* bf16 rows x [R, K]; K a multiple of 8. */
+int sg_fp8_quantize_rows(const void* x_dev, int64_t x_stride, int32_t num_rows, int32_t columns,
+                         const SgFp8RowsOut* out, sg_stream_t stream);
+
+/* sg_add_rmsnorm with the normed rows in e4m3 (args->out_dev unused): the sum is
+ * rounded to bf16 first (the decoder's residual stream), then
+ * (s * rsqrt(mean(s^2) + eps)) * weight stays fp32 until its e4m3 rounding. */
+int sg_add_rmsnorm_fp8(const SgAddRmsNormArgs* args, const SgFp8RowsOut* out,
+                       sg_stream_t stream);
+
+/* sg_silu_mul with the product in e4m3: silu(gate) * up stays fp32 until then. */
+int sg_silu_mul_fp8(const void* gate_up_dev, int64_t gate_up_row_stride, int32_t num_rows,
+                    int32_t intermediate, const SgFp8RowsOut* out, sg_stream_t stream);
+
+/* One-time re-layout of a weight [N, K] e4m3 (rows weight_row_stride bytes apart)
+ * into packed_dev, 16-byte aligned: sg_fp8_packed_bytes(N, K) bytes.  -1 for sizes that are
+ * not supported (N or K below 1, or above 2^24). */
+int64_t sg_fp8_packed_bytes(int32_t n, int32_t k);
+int sg_fp8_pack_weight(const void* weight_dev, int64_t weight_row_stride, int32_t n, int32_t k,
+                       void* packed_dev, sg_stream_t stream);
+
+/* out[r, c] = bf16(sum over 128-column blocks b of
+ *   row_scale[b, r] * weight_scale[c/128, b] * sum_k code[r, k] * weight[c, k]).
+ * Sums are fp32; a block's products are added by the matrix instruction. */
+typedef struct SgFp8MatmulArgs {
+  int32_t num_rows;                /* R */
+  int32_t n;                       /* output columns */
+  int32_t k;                       /* columns of the activations */
+  int32_t reserved;
+  const void* codes_dev;           /* e4m3 [R, code_stride], 16-byte aligned */
+  int64_t code_stride;             /* multiple of 16, >= Kp */
+  const float* scales_dev;         /* [Kp/128, scale_stride] */
+  int64_t scale_stride;
+  const void* weight_dev;          /* packed by sg_fp8_pack_weight */
+  const float* weight_scales_dev;  /* [ceil(N/128), Kp/128] */
+  void* out_dev;                   /* bf16 [R, out_stride], 16-byte aligned */
+  int64_t out_stride;              /* multiple of 8, >= N; columns N .. are not written */
+  void* workspace_dev;             /* sg_fp8_matmul_workspace_bytes(R, N, K) bytes, or NULL
+                                      where that is 0; not shared by overlapping calls */
+  size_t workspace_bytes;
+} SgFp8MatmulArgs;
+
+int64_t sg_fp8_matmul_workspace_bytes(int32_t num_rows, int32_t n, int32_t k);
+int sg_fp8_matmul(const SgFp8MatmulArgs* args, sg_stream_t stream);
+
 /* sizeof() of the argument structs as compiled into the library, for binding
  * checks: which = 0 SgTreeAttnArgs, 1 SgKvCommitArgs, 2 SgTreeSampleArgs,
- * 3 SgKvSplitArgs, 4 SgLmHeadArgs, 5 SgAddRmsNormArgs, 6 SgQkNormRopeArgs.
+ * 3 SgKvSplitArgs, 4 SgLmHeadArgs, 5 SgAddRmsNormArgs, 6 SgQkNormRopeArgs,
+ * 7 SgKvCommitMx4Args, 8 SgTreeAttnMx4Args, 9 SgFp8RowsOut, 10 SgFp8MatmulArgs.
  * Returns -1 for an unknown index.  No reference counterpart. */
 int64_t sg_abi_struct_size(int32_t which);
 

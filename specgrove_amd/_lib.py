@@ -131,6 +131,48 @@ class SgQkNormRopeArgs(ctypes.Structure):
     ]
 
 
+class SgKvCommitMx4Args(ctypes.Structure):
+    _fields_ = [
+        ("num_layers", c_i32), ("num_requests", c_i32), ("num_kv_heads", c_i32),
+        ("head_dim", c_i32),
+        ("k_code_layers_dev", c_void_p), ("k_scale_layers_dev", c_void_p),
+        ("v_code_layers_dev", c_void_p), ("v_scale_layers_dev", c_void_p),
+        ("code_head_stride", c_i64), ("code_token_stride", c_i64),
+        ("scale_head_stride", c_i64), ("scale_token_stride", c_i64),
+        ("k_tree_layers_dev", c_void_p), ("v_tree_layers_dev", c_void_p),
+        ("tree_row_stride", c_i64), ("tree_head_stride", c_i64),
+        ("row_offset_dev", c_void_p), ("keep_rows_dev", c_void_p),
+        ("keep_stride", c_i32), ("keep_len_dev", c_void_p),
+        ("prefix_start_dev", c_void_p), ("lengths_dev", c_void_p),
+        ("capacity", c_i32), ("status_dev", c_void_p),
+    ]
+
+
+class SgTreeAttnMx4Args(ctypes.Structure):
+    _fields_ = [
+        ("attn", SgTreeAttnArgs), ("k_scale_dev", c_void_p), ("v_scale_dev", c_void_p),
+        ("scale_head_stride", c_i64), ("scale_token_stride", c_i64),
+    ]
+
+
+class SgFp8RowsOut(ctypes.Structure):
+    _fields_ = [
+        ("codes_dev", c_void_p), ("code_stride", c_i64),
+        ("scales_dev", c_void_p), ("scale_stride", c_i64),
+    ]
+
+
+class SgFp8MatmulArgs(ctypes.Structure):
+    _fields_ = [
+        ("num_rows", c_i32), ("n", c_i32), ("k", c_i32), ("reserved", c_i32),
+        ("codes_dev", c_void_p), ("code_stride", c_i64),
+        ("scales_dev", c_void_p), ("scale_stride", c_i64),
+        ("weight_dev", c_void_p), ("weight_scales_dev", c_void_p),
+        ("out_dev", c_void_p), ("out_stride", c_i64),
+        ("workspace_dev", c_void_p), ("workspace_bytes", c_size),
+    ]
+
+
 EXPORTED_SYMBOLS = (
     "sg_abi_version", "sg_last_error", "sg_abi_struct_size",
     "sg_tree_attn_plan", "sg_tree_attn_fwd", "sg_kv_commit",
@@ -140,6 +182,10 @@ EXPORTED_SYMBOLS = (
     "sg_lm_head", "sg_lm_head_tile_count", "sg_lm_head_packed", "sg_lm_head_pack_weight",
     "sg_lm_head_packed_bytes", "sg_lm_head_fresh",
     "sg_add_rmsnorm", "sg_qk_norm_rope", "sg_silu_mul", "sg_gather_rows",
+    "sg_kv_commit_mx4", "sg_kv_load_mx4", "sg_tree_attn_mx4_fwd",
+    "sg_fp8_quantize_rows", "sg_add_rmsnorm_fp8", "sg_silu_mul_fp8",
+    "sg_fp8_packed_bytes", "sg_fp8_pack_weight", "sg_fp8_matmul",
+    "sg_fp8_matmul_workspace_bytes",
 )
 
 # Static scratch of sg_tree_sample_noalloc (SG_TREE_SAMPLE_NOALLOC_SCRATCH_BYTES).
@@ -212,6 +258,30 @@ def load() -> ctypes.CDLL:
     lib.sg_gather_rows.restype = c_i32
     lib.sg_gather_rows.argtypes = [c_void_p, c_i32, c_i64, c_i32, c_i32, c_void_p, c_i32,
                                    c_void_p, c_i64, c_void_p, c_void_p]
+    lib.sg_kv_commit_mx4.restype = c_i32
+    lib.sg_kv_commit_mx4.argtypes = [ctypes.POINTER(SgKvCommitMx4Args), c_void_p]
+    lib.sg_kv_load_mx4.restype = c_i32
+    lib.sg_kv_load_mx4.argtypes = [c_void_p, c_i64, c_i64, c_void_p, c_i64, c_i64, c_i32, c_i32,
+                                   c_i32, c_void_p, c_i64, c_i64, c_void_p]
+    lib.sg_tree_attn_mx4_fwd.restype = c_i32
+    lib.sg_tree_attn_mx4_fwd.argtypes = [ctypes.POINTER(SgTreeAttnMx4Args), c_void_p]
+    lib.sg_fp8_quantize_rows.restype = c_i32
+    lib.sg_fp8_quantize_rows.argtypes = [c_void_p, c_i64, c_i32, c_i32,
+                                         ctypes.POINTER(SgFp8RowsOut), c_void_p]
+    lib.sg_add_rmsnorm_fp8.restype = c_i32
+    lib.sg_add_rmsnorm_fp8.argtypes = [ctypes.POINTER(SgAddRmsNormArgs),
+                                       ctypes.POINTER(SgFp8RowsOut), c_void_p]
+    lib.sg_silu_mul_fp8.restype = c_i32
+    lib.sg_silu_mul_fp8.argtypes = [c_void_p, c_i64, c_i32, c_i32,
+                                    ctypes.POINTER(SgFp8RowsOut), c_void_p]
+    lib.sg_fp8_packed_bytes.restype = c_i64
+    lib.sg_fp8_packed_bytes.argtypes = [c_i32, c_i32]
+    lib.sg_fp8_pack_weight.restype = c_i32
+    lib.sg_fp8_pack_weight.argtypes = [c_void_p, c_i64, c_i32, c_i32, c_void_p, c_void_p]
+    lib.sg_fp8_matmul_workspace_bytes.restype = c_i64
+    lib.sg_fp8_matmul_workspace_bytes.argtypes = [c_i32, c_i32, c_i32]
+    lib.sg_fp8_matmul.restype = c_i32
+    lib.sg_fp8_matmul.argtypes = [ctypes.POINTER(SgFp8MatmulArgs), c_void_p]
     lib.sg_clock_probe.restype = c_i32
     lib.sg_clock_probe.argtypes = [c_void_p, c_i32, c_void_p]
     lib.sg_wall_clock_khz.restype = c_i64
@@ -224,7 +294,8 @@ def load() -> ctypes.CDLL:
                            f"version {SG_ABI_VERSION}; rebuild with `python -m "
                            f"specgrove_amd.build`")
     expected = {0: SgTreeAttnArgs, 1: SgKvCommitArgs, 2: SgTreeSampleArgs, 3: SgKvSplitArgs,
-                4: SgLmHeadArgs, 5: SgAddRmsNormArgs, 6: SgQkNormRopeArgs}
+                4: SgLmHeadArgs, 5: SgAddRmsNormArgs, 6: SgQkNormRopeArgs, 7: SgKvCommitMx4Args,
+                8: SgTreeAttnMx4Args, 9: SgFp8RowsOut, 10: SgFp8MatmulArgs}
     for which, struct in expected.items():
         size = lib.sg_abi_struct_size(which)
         if size != ctypes.sizeof(struct):

@@ -31,6 +31,10 @@ extern "C" int64_t sg_abi_struct_size(int32_t which) {
     case 4: return static_cast<int64_t>(sizeof(SgLmHeadArgs));
     case 5: return static_cast<int64_t>(sizeof(SgAddRmsNormArgs));
     case 6: return static_cast<int64_t>(sizeof(SgQkNormRopeArgs));
+    case 7: return static_cast<int64_t>(sizeof(SgKvCommitMx4Args));
+    case 8: return static_cast<int64_t>(sizeof(SgTreeAttnMx4Args));
+    case 9: return static_cast<int64_t>(sizeof(SgFp8RowsOut));
+    case 10: return static_cast<int64_t>(sizeof(SgFp8MatmulArgs));
     default: return -1;
   }
 }

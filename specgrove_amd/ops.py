@@ -832,3 +832,341 @@ def lm_head(hidden: torch.Tensor, weight,
     _lib.check(_lib.load().sg_lm_head_fresh(ctypes.byref(a), int(packed), _stream_handle()),
                "sg_lm_head_packed" if packed else "sg_lm_head")
     return res
+
+
+# --------------------------------------------------------------------------
+# (E) the cache in 4 bits
+# --------------------------------------------------------------------------
+# Rows of D values as codes [..., D/2] and scales [..., D/32] (uint8): e2m1
+# elements, two a byte, with one power-of-two scale for 32 of them (the header
+# says which).  Every value is a bf16 value.
+
+def _check_mx4(codes: torch.Tensor, scales: torch.Tensor, name: str) -> None:
+    _check_device_tensor(codes, f"{name}_codes", torch.uint8)
+    _check_device_tensor(scales, f"{name}_scales", torch.uint8)
+    _require(codes.dim() >= 2 and codes.shape[:-1] == scales.shape[:-1]
+             and codes.shape[-1] == 16 * scales.shape[-1] and scales.shape[-1] >= 1,
+             f"{name}_codes must be [..., tokens, D/2] and {name}_scales [..., tokens, D/32]")
+    _require(codes.stride(-1) == 1 and scales.stride(-1) == 1,
+             f"{name}_codes and {name}_scales must have a contiguous last dimension")
+
+
+def tree_attention_mx4(q: torch.Tensor, k_codes: torch.Tensor, k_scales: torch.Tensor,
+                       v_codes: torch.Tensor, v_scales: torch.Tensor, k_tree: torch.Tensor,
+                       v_tree: torch.Tensor, row_offset: torch.Tensor,
+                       prefix_start: torch.Tensor, prefix_len: torch.Tensor,
+                       parent: torch.Tensor, plan: AttnPlan, out: torch.Tensor | None = None,
+                       scale: float | None = None,
+                       status: torch.Tensor | None = None) -> torch.Tensor:
+    """Packed tree attention of one layer over a 4-bit cache (see
+    prepare_tree_attention_mx4)."""
+    return prepare_tree_attention_mx4(q, k_codes, k_scales, v_codes, v_scales, k_tree, v_tree,
+                                      row_offset, prefix_start, prefix_len, parent, plan, out=out,
+                                      scale=scale, status=status)()
+
+
+def prepare_tree_attention_mx4(q: torch.Tensor, k_codes: torch.Tensor, k_scales: torch.Tensor,
+                               v_codes: torch.Tensor, v_scales: torch.Tensor,
+                               k_tree: torch.Tensor, v_tree: torch.Tensor,
+                               row_offset: torch.Tensor, prefix_start: torch.Tensor,
+                               prefix_len: torch.Tensor, parent: torch.Tensor, plan: AttnPlan,
+                               out: torch.Tensor | None = None, scale: float | None = None,
+                               status: torch.Tensor | None = None) -> PreparedCall:
+    """Packed tree attention of one layer whose prefixes are held in 4 bits,
+    validated and bound (call it to run).
+
+    k/v_codes [Hkv, tokens, D/2] and k/v_scales [Hkv, tokens, D/32] uint8 (the
+    layer's arena, rows written by ``kv_commit_mx4``); everything else, the plan
+    included, as in ``prepare_tree_attention``.  What lies behind a request's
+    last token is not looked at.  An infinity or a NaN in a tree row reaches only
+    the rows that see it; a cached row packed from one gives NaN.
+    """
+    for t, name in ((q, "q"), (k_tree, "k_tree"), (v_tree, "v_tree")):
+        _check_rows(t, name)
+    _check_mx4(k_codes, k_scales, "k")
+    _check_mx4(v_codes, v_scales, "v")
+    _check_device_tensors((row_offset, prefix_len, parent),
+                          ("row_offset", "prefix_len", "parent"), torch.int32)
+    _check_device_tensor(prefix_start, "prefix_start", torch.int64)
+    for t, name in ((row_offset, "row_offset"), (prefix_len, "prefix_len"), (parent, "parent"),
+                    (prefix_start, "prefix_start")):
+        _require(t.is_contiguous(), f"{name} must be contiguous")
+    _require(q.dim() == 3 and k_tree.dim() == 3 and k_codes.dim() == 3,
+             "q/k_tree must be [R, H, D] and k_codes [Hkv, tokens, D/2]")
+    rows, hq, dim = q.shape
+    hkv = k_codes.shape[0]
+    _require(k_codes.shape == v_codes.shape and k_codes.stride() == v_codes.stride()
+             and k_scales.stride() == v_scales.stride(),
+             "k and v codes and scales must share shape and strides")
+    _require(k_codes.shape[2] * 2 == dim, "head dims disagree")
+    _require(not any((t.data_ptr() | t.stride(0) | t.stride(1)) % 16 for t in (k_codes, v_codes)),
+             "codes must be 16-byte aligned, their strides multiples of 16 bytes")
+    _require(k_tree.shape == (rows, hkv, dim) and v_tree.shape == k_tree.shape
+             and k_tree.stride() == v_tree.stride(),
+             "k_tree/v_tree must be [R, Hkv, D] with equal strides")
+    n = prefix_len.numel()
+    check_plan_call(plan, n, rows, hq, hkv, dim)
+    _require(plan.device is not None and plan.device.is_cuda, "plan is not on the device")
+    _require(parent.numel() >= rows, "parent must cover every packed row")
+    _require(row_offset.numel() == n + 1 and prefix_start.numel() == n,
+             "request metadata sizes disagree")
+    if status is not None:
+        _check_device_tensor(status, "status", torch.int32)
+    if out is None:
+        out = torch.empty((rows, hq, dim), dtype=torch.bfloat16, device=q.device)
+    _check_rows(out, "out")
+    _require(out.shape == (rows, hq, dim), "out must be [R, Hq, D]")
+    _check_current(q, "q")
+    workspace = plan.workspace
+    attn = _lib.SgTreeAttnArgs(
+        n, rows, hq, hkv, dim, float(dim ** -0.5 if scale is None else scale),
+        q.data_ptr(), q.stride(0), q.stride(1),
+        k_codes.data_ptr(), v_codes.data_ptr(), k_codes.stride(0), k_codes.stride(1),
+        k_tree.data_ptr(), v_tree.data_ptr(), k_tree.stride(0), k_tree.stride(1),
+        row_offset.data_ptr(), prefix_start.data_ptr(), prefix_len.data_ptr(),
+        parent.data_ptr(), out.data_ptr(), out.stride(0), out.stride(1),
+        plan.device.data_ptr(), plan.host.ctypes.data, plan.units, plan.merges,
+        workspace.data_ptr() if workspace is not None else 0,
+        workspace.numel() if workspace is not None else 0,
+        status.data_ptr() if status is not None else 0)
+    a = _lib.SgTreeAttnMx4Args(attn, k_scales.data_ptr(), v_scales.data_ptr(),
+                               k_scales.stride(0), k_scales.stride(1))
+    keep = (q, k_codes, k_scales, v_codes, v_scales, k_tree, v_tree, row_offset, prefix_start,
+            prefix_len, parent, plan, out, status)
+    return PreparedCall("sg_tree_attn_mx4_fwd", a, keep, result=out)
+
+
+def kv_commit_mx4(k_code_ptrs: torch.Tensor, k_scale_ptrs: torch.Tensor,
+                  v_code_ptrs: torch.Tensor, v_scale_ptrs: torch.Tensor,
+                  k_tree_ptrs: torch.Tensor, v_tree_ptrs: torch.Tensor, **kw) -> None:
+    """Pack the kept rows of every layer into the 4-bit cache (one call; see
+    prepare_kv_commit_mx4)."""
+    prepare_kv_commit_mx4(k_code_ptrs, k_scale_ptrs, v_code_ptrs, v_scale_ptrs, k_tree_ptrs,
+                          v_tree_ptrs, **kw)()
+
+
+def prepare_kv_commit_mx4(k_code_ptrs: torch.Tensor, k_scale_ptrs: torch.Tensor,
+                          v_code_ptrs: torch.Tensor, v_scale_ptrs: torch.Tensor,
+                          k_tree_ptrs: torch.Tensor, v_tree_ptrs: torch.Tensor, *,
+                          num_kv_heads: int, head_dim: int, code_head_stride: int,
+                          code_token_stride: int, scale_head_stride: int,
+                          scale_token_stride: int, tree_row_stride: int, tree_head_stride: int,
+                          row_offset: torch.Tensor, keep_rows: torch.Tensor | None,
+                          keep_len: torch.Tensor, prefix_start: torch.Tensor,
+                          lengths: torch.Tensor, capacity: int,
+                          status: torch.Tensor | None = None) -> PreparedCall:
+    """``prepare_kv_commit`` into a 4-bit arena: the kept bf16 rows of every
+    layer are packed and appended.
+
+    ``*_ptrs`` are int64 device arrays of per-layer base addresses; the strides of
+    codes and scales are in bytes.  ``keep_rows`` [n, keep_stride] i32, or None: a
+    request keeps its rows 0 .. keep_len - 1 (a prefilled prompt).
+    """
+    pointers = (k_code_ptrs, k_scale_ptrs, v_code_ptrs, v_scale_ptrs, k_tree_ptrs, v_tree_ptrs)
+    names = ("k_code_ptrs", "k_scale_ptrs", "v_code_ptrs", "v_scale_ptrs", "k_tree_ptrs",
+             "v_tree_ptrs")
+    _check_device_tensors((*pointers, prefix_start), (*names, "prefix_start"), torch.int64)
+    _check_device_tensors((row_offset, keep_len, lengths),
+                          ("row_offset", "keep_len", "lengths"), torch.int32)
+    for t, name in zip((*pointers, prefix_start, row_offset, keep_len, lengths),
+                       (*names, "prefix_start", "row_offset", "keep_len", "lengths")):
+        _require(t.is_contiguous(), f"{name} must be contiguous")
+    layers = k_code_ptrs.numel()
+    _require(all(t.numel() == layers for t in pointers), "per-layer pointer arrays disagree")
+    n = keep_len.numel()
+    keep_stride = max(1, int(capacity))
+    if keep_rows is not None:
+        _check_device_tensor(keep_rows, "keep_rows", torch.int32)
+        _require(keep_rows.dim() == 2 and keep_rows.is_contiguous(),
+                 "keep_rows must be [n, stride]")
+        _require(keep_rows.shape[0] == n, "request metadata sizes disagree")
+        keep_stride = keep_rows.shape[1]
+    _require(lengths.numel() == n and prefix_start.numel() == n and row_offset.numel() == n + 1,
+             "request metadata sizes disagree")
+    if status is not None:
+        _check_device_tensor(status, "status", torch.int32)
+    _check_current(lengths, "lengths")
+    a = _lib.SgKvCommitMx4Args(
+        layers, n, num_kv_heads, head_dim, *(t.data_ptr() for t in pointers[:4]),
+        code_head_stride, code_token_stride, scale_head_stride, scale_token_stride,
+        k_tree_ptrs.data_ptr(), v_tree_ptrs.data_ptr(), tree_row_stride, tree_head_stride,
+        row_offset.data_ptr(), keep_rows.data_ptr() if keep_rows is not None else 0, keep_stride,
+        keep_len.data_ptr(), prefix_start.data_ptr(), lengths.data_ptr(), capacity,
+        status.data_ptr() if status is not None else 0)
+    keep = (*pointers, row_offset, keep_rows, keep_len, prefix_start, lengths, status)
+    return PreparedCall("sg_kv_commit_mx4", a, keep)
+
+
+def kv_load_mx4(codes: torch.Tensor, scales: torch.Tensor,
+                out: torch.Tensor | None = None) -> torch.Tensor:
+    """bf16 values [..., tokens, D] of packed rows codes [..., tokens, D/2] and
+    scales [..., tokens, D/32] (views of an arena too: the dimensions before the
+    last two must be one stride apart)."""
+    _check_mx4(codes, scales, "cache")
+    dim = 2 * codes.shape[-1]
+    shape = (*codes.shape[:-1], dim)
+    if out is None:
+        out = torch.empty(shape, dtype=torch.bfloat16, device=codes.device)
+    _check_rows(out, "out")
+    _require(tuple(out.shape) == shape, "out must be [..., tokens, D]")
+    if out.numel() == 0:
+        return out
+    flat = []
+    for t, name in ((codes, "codes"), (scales, "scales"), (out, "out")):
+        try:
+            flat.append(t.view(-1, *t.shape[-2:]))
+        except RuntimeError:
+            raise ValueError(f"{name}: the dimensions before the last two must be one stride "
+                             f"apart") from None
+    c, s, o = flat
+    _require(not (c.data_ptr() | c.stride(0) | c.stride(1)) % 4,
+             "codes must be 4-byte aligned, their strides multiples of 4 bytes")
+    _check_current(codes, "codes")
+    _lib.check(_lib.load().sg_kv_load_mx4(
+        c.data_ptr(), c.stride(0), c.stride(1), s.data_ptr(), s.stride(0), s.stride(1),
+        c.shape[0], c.shape[1], dim, o.data_ptr(), o.stride(0), o.stride(1), _stream_handle()),
+        "sg_kv_load_mx4")
+    return out
+
+
+# --------------------------------------------------------------------------
+# (F) projections in 8-bit floating point
+# --------------------------------------------------------------------------
+
+FP8_BLOCK = 128  # columns (and weight rows) of a scale
+
+
+@dataclass
+class Fp8Rows:
+    """Activation rows in e4m3 with an fp32 scale for each row and 128 columns."""
+    codes: torch.Tensor   # [R, K] float8_e4m3fn, a view of rows padded with zeros to 128 columns
+    scales: torch.Tensor  # [R, ceil(K/128)] f32, a view of [ceil(K/128), R]
+
+    @property
+    def shape(self) -> torch.Size:
+        return self.codes.shape
+
+    def dequantize(self) -> torch.Tensor:
+        """The values the rows stand for, [R, K] f32."""
+        k = self.codes.shape[1]
+        return self.codes.float() * self.scales.repeat_interleave(FP8_BLOCK, 1)[:, :k]
+
+
+def _new_fp8_rows(rows: int, columns: int, device) -> "tuple[Fp8Rows, _lib.SgFp8RowsOut]":
+    padded = (columns + FP8_BLOCK - 1) // FP8_BLOCK * FP8_BLOCK
+    codes = torch.empty((rows, padded), dtype=torch.float8_e4m3fn, device=device)
+    scales = torch.empty((padded // FP8_BLOCK, rows), dtype=torch.float32, device=device)
+    out = _lib.SgFp8RowsOut(codes.data_ptr(), padded, scales.data_ptr(), rows)
+    return Fp8Rows(codes[:, :columns], scales.T), out
+
+
+def _check_current(t: torch.Tensor, name: str) -> None:
+    _require(t.device.index == torch.cuda.current_device(),
+             f"{name} is on {t.device}, which is not the current device")
+
+
+def quantize_fp8(x: torch.Tensor) -> Fp8Rows:
+    """bf16 rows [R, K] in e4m3 with a scale for each row and 128 columns (K a
+    multiple of 8, rows 16-byte aligned)."""
+    _check_rows(x, "x")
+    _require(x.dim() == 2, "x must be [R, K]")
+    _check_current(x, "x")
+    rows, out = _new_fp8_rows(x.shape[0], x.shape[1], x.device)
+    _lib.check(_lib.load().sg_fp8_quantize_rows(x.data_ptr(), x.stride(0), x.shape[0], x.shape[1],
+                                                ctypes.byref(out), _stream_handle()),
+               "sg_fp8_quantize_rows")
+    return rows
+
+
+def quantize_fp8_weight(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """A weight [N, K] as e4m3 codes [N, K] and fp32 scales [ceil(N/128),
+    ceil(K/128)], the largest magnitude of a block at 448.  Once per weight, in
+    torch operations, on any device."""
+    _require(weight.dim() == 2 and weight.numel() > 0, "weight must be a matrix")
+    n, k = weight.shape
+    pad = torch.nn.functional.pad(weight.float(), (0, -k % FP8_BLOCK, 0, -n % FP8_BLOCK))
+    blocks = pad.unflatten(0, (-1, FP8_BLOCK)).unflatten(-1, (-1, FP8_BLOCK))
+    most = blocks.abs().amax((1, 3)).clamp_min(2.0 ** -100)
+    codes = (blocks * (448.0 / most)[:, None, :, None]).to(torch.float8_e4m3fn)
+    return (codes.flatten(2).flatten(0, 1)[:n, :k].contiguous(), most / 448.0)
+
+
+class PackedFp8Weight:
+    """An e4m3 weight [N, K] and its block scales, re-laid out once for
+    ``fp8_matmul`` (the order in which the matrix instruction takes it)."""
+    __slots__ = ("packed", "scales", "shape", "device")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
+        _check_device_tensor(codes, "codes", torch.float8_e4m3fn)
+        _require(codes.dim() == 2 and codes.numel() > 0 and codes.stride(1) == 1
+                 and codes.stride(0) >= codes.shape[1], "codes must be a row-contiguous matrix")
+        _check_device_tensor(scales, "scales", torch.float32)
+        n, k = codes.shape
+        _require(tuple(scales.shape) == (-(-n // FP8_BLOCK), -(-k // FP8_BLOCK)),
+                 "scales must be [ceil(N/128), ceil(K/128)]")
+        _require(scales.device == codes.device, "codes and scales must be on one device")
+        _check_current(codes, "codes")
+        lib = _lib.load()
+        nbytes = int(lib.sg_fp8_packed_bytes(n, k))
+        _require(nbytes > 0, "weight size unsupported (N and K up to 2^24)")
+        self.packed = torch.empty(nbytes, dtype=torch.uint8, device=codes.device)
+        self.scales = scales.contiguous().clone()
+        self.shape = torch.Size((n, k))
+        self.device = codes.device
+        _lib.check(lib.sg_fp8_pack_weight(codes.data_ptr(), codes.stride(0), n, k,
+                                          self.packed.data_ptr(), _stream_handle()),
+                   "sg_fp8_pack_weight")
+
+
+def pack_fp8_weight(codes: torch.Tensor, scales: torch.Tensor) -> PackedFp8Weight:
+    """One-time packing of an e4m3 weight (``quantize_fp8_weight``, or a checkpoint
+    with 128 x 128 block scales) for ``fp8_matmul``, enqueued on torch's current
+    stream."""
+    return PackedFp8Weight(codes, scales)
+
+
+def fp8_matmul(rows: Fp8Rows, weight: PackedFp8Weight,
+               out: torch.Tensor | None = None) -> torch.Tensor:
+    """rows @ weight.T in bf16, [R, N]: e4m3 products, fp32 sums, each block of 128
+    columns scaled by its row's and its weight block's scale.
+
+    ``out`` (optional) is a bf16 [R, N] tensor with 16-byte aligned rows.  Without
+    it the result is a view of rows padded to 8 columns.
+    """
+    _require(isinstance(rows, Fp8Rows) and isinstance(weight, PackedFp8Weight),
+             "fp8_matmul takes Fp8Rows and a PackedFp8Weight")
+    codes, scales = rows.codes, rows.scales
+    _check_device_tensor(codes, "codes", torch.float8_e4m3fn)
+    _check_device_tensor(scales, "scales", torch.float32)
+    n, k = weight.shape
+    count = codes.shape[0]
+    blocks = -(-k // FP8_BLOCK)
+    _require(codes.dim() == 2 and codes.shape[1] == k, "rows and weight disagree on K")
+    _require(tuple(scales.shape) == (count, blocks) and (scales.stride(0) == 1 or count == 1),
+             "scales must be the [R, ceil(K/128)] view of the quantized rows")
+    _require(codes.device == weight.device and scales.device == codes.device,
+             "rows and weight must be on one device")
+    _check_current(codes, "rows")
+    # The padded columns behind a row are read: they must be there.
+    behind = codes.untyped_storage().nbytes() - codes.storage_offset()
+    _require(count == 0 or (codes.stride(1) == 1 and codes.stride(0) >= FP8_BLOCK * blocks
+                            and behind >= (count - 1) * codes.stride(0) + FP8_BLOCK * blocks),
+             "codes must be rows padded with zeros to 128 columns")
+    if out is None:
+        out = torch.empty((count, (n + 7) // 8 * 8), dtype=torch.bfloat16,
+                          device=codes.device)[:, :n]
+    else:
+        _check_rows(out, "out")
+        _require(tuple(out.shape) == (count, n) and out.device == codes.device,
+                 "out must be [R, N] on the rows' device")
+    lib = _lib.load()
+    nbytes = int(lib.sg_fp8_matmul_workspace_bytes(count, n, k))
+    workspace = (torch.empty(nbytes, dtype=torch.uint8, device=codes.device)
+                 if nbytes > 0 else None)
+    a = _lib.SgFp8MatmulArgs(
+        count, n, k, 0, codes.data_ptr(), codes.stride(0), scales.data_ptr(),
+        scales.stride(1) if blocks > 1 else max(count, 1), weight.packed.data_ptr(),
+        weight.scales.data_ptr(), out.data_ptr(), out.stride(0),
+        workspace.data_ptr() if workspace is not None else 0, max(nbytes, 0))
+    _lib.check(lib.sg_fp8_matmul(ctypes.byref(a), _stream_handle()), "sg_fp8_matmul")
+    return out

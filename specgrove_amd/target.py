@@ -93,6 +93,48 @@ def silu_mul(gate_up: torch.Tensor) -> torch.Tensor:
     return out
 
 
+def add_rmsnorm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float,
+                    residual: torch.Tensor | None = None, want_sum: bool = False):
+    """``add_rmsnorm`` with the normed rows in e4m3 (``ops.Fp8Rows``), rounded from
+    fp32; with ``want_sum`` also x + residual (bf16 [R, H])."""
+    ops._check_rows(x, "x")
+    ops._require(x.dim() == 2, "x must be [R, H]")
+    rows, hidden = x.shape
+    ops._check_rows(weight, "weight")
+    ops._require(tuple(weight.shape) == (hidden,), "weight must be [H]")
+    if residual is not None:
+        ops._check_rows(residual, "residual")
+        ops._require(residual.shape == x.shape, "residual must be [R, H]")
+    ops._check_current(x, "x")
+    normed, out = ops._new_fp8_rows(rows, hidden, x.device)
+    total = (torch.empty((rows, hidden), dtype=x.dtype, device=x.device) if want_sum else None)
+    a = _lib.SgAddRmsNormArgs()
+    a.num_rows, a.hidden, a.eps = rows, hidden, float(eps)
+    a.x_dev, a.x_stride = x.data_ptr(), x.stride(0)
+    if residual is not None:
+        a.residual_dev, a.residual_stride = residual.data_ptr(), residual.stride(0)
+    a.weight_dev = weight.data_ptr()
+    if total is not None:
+        a.residual_out_dev, a.residual_out_stride = total.data_ptr(), total.stride(0)
+    _lib.check(_lib.load().sg_add_rmsnorm_fp8(ctypes.byref(a), ctypes.byref(out), _stream()),
+               "sg_add_rmsnorm_fp8")
+    return (normed, total) if want_sum else normed
+
+
+def silu_mul_fp8(gate_up: torch.Tensor) -> ops.Fp8Rows:
+    """``silu_mul`` with the product in e4m3 (``ops.Fp8Rows``), rounded from fp32."""
+    ops._check_rows(gate_up, "gate_up")
+    ops._require(gate_up.dim() == 2 and gate_up.shape[1] % 16 == 0,
+                 "gate_up must be [R, 2 I], I a multiple of 8")
+    ops._check_current(gate_up, "gate_up")
+    rows, width = gate_up.shape
+    product, out = ops._new_fp8_rows(rows, width // 2, gate_up.device)
+    _lib.check(_lib.load().sg_silu_mul_fp8(gate_up.data_ptr(), gate_up.stride(0), rows,
+                                           width // 2, ctypes.byref(out), _stream()),
+               "sg_silu_mul_fp8")
+    return product
+
+
 def gather_rows(sources: Sequence[torch.Tensor], index: torch.Tensor) -> torch.Tensor:
     """[K, L*H]: the rows ``index`` of each [R, H] source, side by side."""
     first = sources[0]
