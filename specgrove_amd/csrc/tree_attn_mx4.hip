@@ -45,8 +45,22 @@ __device__ __forceinline__ uint32_t nonfinite_halves(uint32_t w) {
   return lo | hi;
 }
 
+// LDS of a workgroup: two stages of K and two of V (the merge scratch and the
+// output staging after the last window), and the tree's tables.
 template <int D>
-__device__ __forceinline__ void attn_unit_mx4(const SgTreeAttnMx4Args& args, const AttnUnit& u) {
+struct Shared {
+  __align__(1024) unsigned char ring[4 * 2 * kTileKeys * D * 2];
+  uint32_t anc[kQPerUnit][kAncWords];
+  int2 run[kMaxTreeRows];
+  uint32_t odd[kAncWords];  // blocks of 32 tree rows with a V that is no number
+};
+
+// One unit.  kTwo: of 1-2 q-groups; two waves share one and take a 32-key block of
+// each window (key streams, merged at the end).  Otherwise (3-4) a wave takes
+// both blocks.
+template <int D, bool kTwo>
+__device__ __forceinline__ void attn_unit_mx4(const SgTreeAttnMx4Args& args, const AttnUnit& u,
+                                              Shared<D>& sh) {
   const SgTreeAttnArgs& a = args.attn;
   constexpr int KB = D / 16;                  // QK^T k-blocks of 16 head dims
   constexpr int DB = D / 32;                  // PV blocks of 32 head dims
@@ -58,19 +72,21 @@ __device__ __forceinline__ void attn_unit_mx4(const SgTreeAttnMx4Args& args, con
   constexpr int kSlotBytes = STATE * 64 * 4;
   constexpr int kRowBytes = 2 * D;
   constexpr int kPitch = kRowBytes + 16;
-  // Two stages of K, two of V; the merge scratch and the output staging after.
-  __shared__ __align__(1024) unsigned char s_ring[4 * STAGEB];
-  __shared__ uint32_t s_anc[kQPerUnit][kAncWords];
-  __shared__ int2 s_run[kMaxTreeRows];
-  __shared__ uint32_t s_odd[2];  // tree window: its 32-key blocks with a non-finite V
   static_assert(2 * kSlotBytes + 2 * 32 * kPitch <= 4 * STAGEB &&
                     4 * 32 * kPitch <= 4 * STAGEB,
                 "merge scratch and output staging must fit the ring");
+  unsigned char* const s_ring = sh.ring;
+  uint32_t(*const s_anc)[kAncWords] = sh.anc;
+  uint32_t* const s_odd = sh.odd;
   unsigned char* const s_k = s_ring;
   unsigned char* const s_v = s_ring + 2 * STAGEB;
 
   const int G = a.num_q_heads / a.num_kv_heads;
-  const int tid = threadIdx.x;
+  // Opaque, so that what follows from it is not kept in registers from one unit
+  // of a list to the next (83 registers spilled, and a spill's reload waits for
+  // the loads in flight).
+  int tid = threadIdx.x;
+  asm volatile("" : "+v"(tid));
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int half = lane >> 5;
@@ -85,10 +101,8 @@ __device__ __forceinline__ void attn_unit_mx4(const SgTreeAttnMx4Args& args, con
     poison_unit<D>(a, u, r0);
     return;
   }
-  // With 1-2 q-groups two waves share one and take a 32-key block of each window
-  // (key streams, merged at the end); with 3-4 a wave takes both blocks.
   const int nq = (u.row_count * G + 31) / 32;
-  const int streams = nq <= 2 ? 2 : 1;
+  constexpr int streams = kTwo ? 2 : 1;
   const int qg = wave % nq;
   const int ks = wave / nq;
   const bool active = ks < streams;
@@ -101,25 +115,20 @@ __device__ __forceinline__ void attn_unit_mx4(const SgTreeAttnMx4Args& args, con
   const bool do_tree = (u.flags & 1) != 0;
 
   // Pieces of this thread: key row and 32-value block of the window, K or V.
+  // A window's base is scalar, a piece's offset one register for K and V.
+  constexpr int kBlocks = D / 32;             // 32-value blocks of a row
   const int prefix_keys = u.key_end - u.key_begin;
   const int windows = (prefix_keys + kWindow - 1) / kWindow;
+  const int full = prefix_keys / kWindow;
   const int64_t prefix0 = a.prefix_start_dev[u.req] + u.key_begin;
-  const unsigned char* codes[2];
-  const unsigned char* scales[2];
-  codes[0] = static_cast<const unsigned char*>(a.k_cache_dev);
-  codes[1] = static_cast<const unsigned char*>(a.v_cache_dev);
-  scales[0] = static_cast<const unsigned char*>(args.k_scale_dev);
-  scales[1] = static_cast<const unsigned char*>(args.v_scale_dev);
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    codes[t] += g * a.cache_head_stride + prefix0 * a.cache_token_stride;
-    scales[t] += g * args.scale_head_stride + prefix0 * args.scale_token_stride;
-  }
-  constexpr int kBlocks = D / 32;             // 32-value blocks of a row
+  const int64_t code0 = g * a.cache_head_stride + prefix0 * a.cache_token_stride;
+  const int64_t scale0 = g * args.scale_head_stride + prefix0 * args.scale_token_stride;
   const int piece = D == 128 ? tid : tid & 127;
   const int p_row = piece / kBlocks;
   const int p_blk = piece % kBlocks;
-  auto is_v_of = [&](int i) { return D == 128 ? i : wave >> 1; };
+  const bool v_wave = wave >= kThreads / 128;  // D = 64: the upper waves move V
+  const uint32_t c_lane = p_row * static_cast<uint32_t>(a.cache_token_stride) + 16 * p_blk;
+  const uint32_t s_lane = p_row * static_cast<uint32_t>(args.scale_token_stride) + p_blk;
   struct Raw {
     uint4 code[LOADS];
     uint32_t scale[LOADS];
@@ -127,31 +136,43 @@ __device__ __forceinline__ void attn_unit_mx4(const SgTreeAttnMx4Args& args, con
   // Window w of the prefix into registers.  Keys past the range read the last
   // valid one: its score is masked, its probability 0.
   auto load = [&](int w, Raw& r) {
-    const int key = min(w * kWindow + p_row, prefix_keys - 1);
+    uint32_t c_off = c_lane, s_off = s_lane;
+    if (w >= full) {
+      const int key = min(p_row, prefix_keys - 1 - w * kWindow);
+      c_off = key * static_cast<uint32_t>(a.cache_token_stride) + 16 * p_blk;
+      s_off = key * static_cast<uint32_t>(args.scale_token_stride) + p_blk;
+    }
+    const int64_t cb = code0 + static_cast<int64_t>(w) * kWindow * a.cache_token_stride;
+    const int64_t sb = scale0 + static_cast<int64_t>(w) * kWindow * args.scale_token_stride;
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      const int t = is_v_of(i);
-      r.code[i] = *reinterpret_cast<const uint4*>(
-          codes[t] + key * a.cache_token_stride + 16 * p_blk);
-      r.scale[i] = scales[t][key * args.scale_token_stride + p_blk];
+      const bool is_v = D == 128 ? i == 1 : v_wave;
+      const unsigned char* c =
+          static_cast<const unsigned char*>(is_v ? a.v_cache_dev : a.k_cache_dev) + cb;
+      const unsigned char* b =
+          static_cast<const unsigned char*>(is_v ? args.v_scale_dev : args.k_scale_dev) + sb;
+      r.code[i] = *reinterpret_cast<const uint4*>(c + c_off);
+      r.scale[i] = b[s_off];
     }
   };
-  // LDS address of the piece's 16-byte chunk c (of its four) in stage `stage`.
+  // LDS offsets of the piece's first 16-byte chunk (of four) in stage 0 of K and
+  // V.  The swizzles are XORs of the chunk index, so chunk c is at that ^ 16 c.
   const int k_row = (p_row & 32) + key_slot(p_row & 31);
-  auto chunk_at = [&](int t, int stage, int c) {
-    const int chunk = 4 * p_blk + c;
-    return t == 0 ? s_k + stage * STAGEB + k_row * ROWB + 16 * (chunk ^ swz_k<D>(k_row))
-                  : s_v + stage * STAGEB + p_row * ROWB + 16 * (chunk ^ swz_v<D>(p_row));
+  const uint32_t k_at = k_row * ROWB + 16 * ((4 * p_blk) ^ swz_k<D>(k_row));
+  const uint32_t v_at = p_row * ROWB + 16 * ((4 * p_blk) ^ swz_v<D>(p_row));
+  const uint32_t one_at = v_wave ? v_at + 2 * STAGEB : k_at;  // D = 64
+  auto piece_at = [&](int i, int c) {
+    return s_ring + (D == 128 ? (i == 1 ? (v_at ^ (16 * c)) + 2 * STAGEB : k_at ^ (16 * c))
+                              : one_at ^ (16 * c));
   };
   auto unpack = [&](const Raw& r, int stage) {
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      const int t = is_v_of(i);
       const float s = __uint_as_float(r.scale[i] << 23);  // 255: converts to NaN
-      *reinterpret_cast<uint4*>(chunk_at(t, stage, 0)) = unpack8(r.code[i].x, s);
-      *reinterpret_cast<uint4*>(chunk_at(t, stage, 1)) = unpack8(r.code[i].y, s);
-      *reinterpret_cast<uint4*>(chunk_at(t, stage, 2)) = unpack8(r.code[i].z, s);
-      *reinterpret_cast<uint4*>(chunk_at(t, stage, 3)) = unpack8(r.code[i].w, s);
+      const uint32_t w[4] = {r.code[i].x, r.code[i].y, r.code[i].z, r.code[i].w};
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        *reinterpret_cast<uint4*>(piece_at(i, c) + stage * STAGEB) = unpack8(w[c], s);
     }
   };
   // raw[p] holds window w with w & 1 == p.
@@ -159,7 +180,8 @@ __device__ __forceinline__ void attn_unit_mx4(const SgTreeAttnMx4Args& args, con
   if (windows > 0) load(0, raw[0]);
   if (windows > 1) load(1, raw[1]);
 
-  if (do_tree) build_ancestors(a, u, r0, n, s_run, s_anc);
+  if (tid < kAncWords) s_odd[tid] = 0u;  // published by the barriers of what follows
+  if (do_tree) build_ancestors(a, u, r0, n, sh.run, s_anc);
 
   // Query operand: lane supplies Q[row, head, 16*kb + 8*half .. +7].
   bf16x8 qf[KB];
@@ -273,33 +295,28 @@ __device__ __forceinline__ void attn_unit_mx4(const SgTreeAttnMx4Args& args, con
   // their children: no row of the unit sees a tree key behind its last row.
   if (do_tree) {
     const int tree_keys = u.row_begin + u.row_count;
-    const uint16_t* tree[2] = {
-        static_cast<const uint16_t*>(a.k_tree_dev) + g * a.tree_head_stride +
-            static_cast<int64_t>(r0) * a.tree_row_stride,
-        static_cast<const uint16_t*>(a.v_tree_dev) + g * a.tree_head_stride +
-            static_cast<int64_t>(r0) * a.tree_row_stride};
+    const int64_t tree0 = g * a.tree_head_stride + static_cast<int64_t>(r0) * a.tree_row_stride;
     for (int key0 = 0; key0 < tree_keys; key0 += kWindow) {
       const int key = min(key0 + p_row, n - 1);
       uint4 v[LOADS][4];
 #pragma unroll
-      for (int i = 0; i < LOADS; ++i)
+      for (int i = 0; i < LOADS; ++i) {
+        const bool is_v = D == 128 ? i == 1 : v_wave;
+        const uint16_t* src = static_cast<const uint16_t*>(is_v ? a.v_tree_dev : a.k_tree_dev) +
+                              tree0 + static_cast<int64_t>(key) * a.tree_row_stride + 32 * p_blk;
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
-          v[i][c] = *reinterpret_cast<const uint4*>(
-              tree[is_v_of(i)] + static_cast<int64_t>(key) * a.tree_row_stride +
-              8 * (4 * p_blk + c));
+        for (int c = 0; c < 4; ++c) v[i][c] = *reinterpret_cast<const uint4*>(src + 8 * c);
+      }
       __syncthreads();  // the stage is free; s_anc is built
-      if (tid < 2) s_odd[tid] = 0u;
-      __syncthreads();
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
-        const int t = is_v_of(i);
+        const bool is_v = D == 128 ? i == 1 : v_wave;
         uint32_t any = 0u;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          if (t == 1) {
+          if (is_v) {
             // A value that is no number would reach every row of the block
-            // through a product with 0: it is added by itself below.
+            // through a product with 0: it is added by itself at the end.
             uint32_t w[4] = {v[i][c].x, v[i][c].y, v[i][c].z, v[i][c].w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -309,29 +326,16 @@ __device__ __forceinline__ void attn_unit_mx4(const SgTreeAttnMx4Args& args, con
             }
             v[i][c] = make_uint4(w[0], w[1], w[2], w[3]);
           }
-          *reinterpret_cast<uint4*>(chunk_at(t, 0, c)) = v[i][c];
+          *reinterpret_cast<uint4*>(piece_at(i, c)) = v[i][c];
         }
-        if (any != 0u) s_odd[p_row >> 5] = 1u;
+        if (any != 0u) s_odd[(key0 + p_row) >> 5] = 1u;
       }
       __syncthreads();
       if (!active) continue;
       for (int b = streams == 2 ? ks : 0; b < (streams == 2 ? ks + 1 : 2); ++b) {
         const int first = key0 + 32 * b;
         if (first >= tree_keys) break;
-        const uint32_t word = s_anc[r_local][first >> 5];
-        block(qk(b * TILEB), b * TILEB, n - first, word >> (16 * half));
-        if (s_odd[b] == 0u) continue;
-        for (int j = 0; j < 32 && first + j < n; ++j) {
-          const uint16_t* vr = tree[1] + static_cast<int64_t>(first + j) * a.tree_row_stride;
-          const bool sees = ((word >> j) & 1u) != 0u;
-#pragma unroll
-          for (int db = 0; db < DB; ++db)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              const uint16_t h = vr[32 * db + 8 * (r >> 2) + 4 * half + (r & 3)];
-              if (sees && (h & 0x7f80u) == 0x7f80u) st.acc[db][r] += bf16_to_f32(h);
-            }
-        }
+        block(qk(b * TILEB), b * TILEB, n - first, s_anc[r_local][first >> 5] >> (16 * half));
       }
     }
     __syncthreads();  // stage 0 is free
@@ -339,33 +343,12 @@ __device__ __forceinline__ void attn_unit_mx4(const SgTreeAttnMx4Args& args, con
 
   // The prefix.  Window w is read from stage w & 1 while window w + 1 is
   // unpacked into the other one and w + 2 and w + 3 are on their way.
-  auto compute = [&](int stage, int left) {
-    const int at = stage * STAGEB;
-    if (left >= kWindow) {
-      if (streams == 2) {
-        const floatx16 s = qk(at + ks * TILEB);
-        float x[16];
+  auto whole_block = [&](const floatx16& s, int at) {
+    float x[16];
 #pragma unroll
-        for (int r = 0; r < 16; ++r) x[r] = s[r];
-        softmax(x);
-        pv(x, at + ks * TILEB);
-      } else {
-        const floatx16 s0 = qk(at);
-        const floatx16 s1 = qk(at + TILEB);
-        float x[16];
-#pragma unroll
-        for (int r = 0; r < 16; ++r) x[r] = s0[r];
-        softmax(x);
-        pv(x, at);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) x[r] = s1[r];
-        softmax(x);
-        pv(x, at + TILEB);
-      }
-    } else {
-      for (int b = streams == 2 ? ks : 0; b < (streams == 2 ? ks + 1 : 2); ++b)
-        if (32 * b < left) block(qk(at + b * TILEB), at + b * TILEB, left - 32 * b, 0xffffu);
-    }
+    for (int r = 0; r < 16; ++r) x[r] = s[r];
+    softmax(x);
+    pv(x, at);
   };
   auto step = [&](int w, auto parity) {
     constexpr int p = decltype(parity)::value;  // w & 1
@@ -374,7 +357,17 @@ __device__ __forceinline__ void attn_unit_mx4(const SgTreeAttnMx4Args& args, con
       unpack(raw[1 - p], 1 - p);
       if (w + 3 < windows) load(w + 3, raw[1 - p]);
     }
-    if (active) compute(p, prefix_keys - w * kWindow);
+    if (w == full || !active) return;
+    constexpr int at = p * STAGEB;
+    if constexpr (kTwo) {
+      const int mine = at + ks * TILEB;
+      whole_block(qk(mine), mine);
+    } else {
+      const floatx16 s0 = qk(at);
+      const floatx16 s1 = qk(at + TILEB);
+      whole_block(s0, at);
+      whole_block(s1, at + TILEB);
+    }
   };
   if (windows > 0) {
     unpack(raw[0], 0);
@@ -383,6 +376,13 @@ __device__ __forceinline__ void attn_unit_mx4(const SgTreeAttnMx4Args& args, con
   for (int w = 0; w < windows; w += 2) {
     step(w, std::integral_constant<int, 0>{});
     if (w + 1 < windows) step(w + 1, std::integral_constant<int, 1>{});
+  }
+  if (windows > full && active) {  // the last window, of fewer keys
+    const int left = prefix_keys - full * kWindow;
+    for (int b = streams == 2 ? ks : 0; b < (streams == 2 ? ks + 1 : 2); ++b) {
+      const int at = (full & 1) * STAGEB + b * TILEB;
+      if (32 * b < left) block(qk(at), at, left - 32 * b, 0xffffu);
+    }
   }
   __syncthreads();
 
@@ -417,6 +417,32 @@ __device__ __forceinline__ void attn_unit_mx4(const SgTreeAttnMx4Args& args, con
   }
 
   // st.acc[db][r] holds head dim 32*db + 8*(r/4) + 4*half + (r%4) of this lane's query.
+  if (do_tree) {
+    const uint16_t* vt = static_cast<const uint16_t*>(a.v_tree_dev) + g * a.tree_head_stride +
+                         static_cast<int64_t>(r0) * a.tree_row_stride + 4 * half;
+    for (int t = 0; t < kAncWords; ++t) {
+      if (s_odd[t] == 0u) continue;
+      const uint32_t word = s_anc[r_local][t];
+#pragma unroll 1
+      for (int j = 0; j < 32 && 32 * t + j < n; ++j) {
+        const uint16_t* vr = vt + static_cast<int64_t>(32 * t + j) * a.tree_row_stride;
+        const bool sees = ((word >> j) & 1u) != 0u;
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+          for (int q4 = 0; q4 < 4; ++q4) {
+            const uint2 v = *reinterpret_cast<const uint2*>(vr + 32 * db + 8 * q4);
+            const uint32_t w[2] = {v.x, v.y};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t h = (w[e >> 1] >> (16 * (e & 1))) & 0xffffu;
+              if (sees && (h & 0x7f80u) == 0x7f80u)
+                st.acc[db][4 * q4 + e] += __uint_as_float(h << 16);
+            }
+          }
+      }
+    }
+  }
   if (u.partial >= 0) {
     // Partial layout (floats): O as float4 chunks ((db*4 + q4)*2 + half)*128 + m,
     // then the running max (log2 units) and sum per query vector.
@@ -491,6 +517,8 @@ __device__ __forceinline__ void attn_unit_mx4(const SgTreeAttnMx4Args& args, con
 template <int D>
 __global__ __launch_bounds__(kThreads, 2) void tree_attn_mx4_kernel(SgTreeAttnMx4Args a,
                                                                      const AttnUnit* direct) {
+  __shared__ Shared<D> sh;
+  const int group = a.attn.num_q_heads / a.attn.num_kv_heads;
   const AttnUnit* units = direct;
   int k = blockIdx.x;
   int end = k + 1;
@@ -504,7 +532,11 @@ __global__ __launch_bounds__(kThreads, 2) void tree_attn_mx4_kernel(SgTreeAttnMx
   }
   for (; k < end; ++k) {
     const AttnUnit u = units[k];
-    attn_unit_mx4<D>(a, u);
+    if (u.row_count * group <= 64) {
+      attn_unit_mx4<D, true>(a, u, sh);
+    } else {
+      attn_unit_mx4<D, false>(a, u, sh);
+    }
     __syncthreads();  // LDS of this unit is free before the next one starts
   }
 }
@@ -525,8 +557,10 @@ extern "C" int sg_tree_attn_mx4_fwd(const SgTreeAttnMx4Args* args, sg_stream_t s
                  ((reinterpret_cast<uintptr_t>(a.k_cache_dev) |
                    reinterpret_cast<uintptr_t>(a.v_cache_dev)) & 15) == 0,
              "codes must be 16-byte aligned, their strides multiples of 16 bytes");
-  SG_REQUIRE(a.cache_token_stride >= 0 && args->scale_token_stride >= 0,
-             "token strides must not be negative");
+  // Offsets inside a window are 32-bit.
+  SG_REQUIRE(a.cache_token_stride >= 0 && a.cache_token_stride < (int64_t{1} << 24) &&
+                 args->scale_token_stride >= 0 && args->scale_token_stride < (int64_t{1} << 24),
+             "token strides must lie in [0, 2^24) bytes");
   const hipStream_t s = static_cast<hipStream_t>(stream);
   if (a.head_dim == 128) {
     tree_attn_mx4_kernel<128><<<dim3(a.plan_units), dim3(kThreads), 0, s>>>(*args, call.direct);

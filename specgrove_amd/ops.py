@@ -860,9 +860,12 @@ def tree_attention_mx4(q: torch.Tensor, k_codes: torch.Tensor, k_scales: torch.T
                        status: torch.Tensor | None = None) -> torch.Tensor:
     """Packed tree attention of one layer over a 4-bit cache (see
     prepare_tree_attention_mx4)."""
-    return prepare_tree_attention_mx4(q, k_codes, k_scales, v_codes, v_scales, k_tree, v_tree,
-                                      row_offset, prefix_start, prefix_len, parent, plan, out=out,
-                                      scale=scale, status=status)()
+    args, out = _mx4_attention_args(q, k_codes, k_scales, v_codes, v_scales, k_tree, v_tree,
+                                    row_offset, prefix_start, prefix_len, parent, plan, out,
+                                    scale, status)
+    _lib.check(_lib.load().sg_tree_attn_mx4_fwd(ctypes.byref(args), _stream_handle()),
+               "sg_tree_attn_mx4_fwd")
+    return out
 
 
 def prepare_tree_attention_mx4(q: torch.Tensor, k_codes: torch.Tensor, k_scales: torch.Tensor,
@@ -881,6 +884,17 @@ def prepare_tree_attention_mx4(q: torch.Tensor, k_codes: torch.Tensor, k_scales:
     last token is not looked at.  An infinity or a NaN in a tree row reaches only
     the rows that see it; a cached row packed from one gives NaN.
     """
+    args, out = _mx4_attention_args(q, k_codes, k_scales, v_codes, v_scales, k_tree, v_tree,
+                                    row_offset, prefix_start, prefix_len, parent, plan, out,
+                                    scale, status)
+    keep = (q, k_codes, k_scales, v_codes, v_scales, k_tree, v_tree, row_offset, prefix_start,
+            prefix_len, parent, plan, out, status)
+    return PreparedCall("sg_tree_attn_mx4_fwd", args, keep, result=out)
+
+
+def _explain_mx4_attention(q, k_codes, k_scales, v_codes, v_scales, k_tree, v_tree, row_offset,
+                           prefix_start, prefix_len, parent, plan, out, status) -> None:
+    """Raise ValueError for the first argument that does not fit."""
     for t, name in ((q, "q"), (k_tree, "k_tree"), (v_tree, "v_tree")):
         _check_rows(t, name)
     _check_mx4(k_codes, k_scales, "k")
@@ -893,47 +907,95 @@ def prepare_tree_attention_mx4(q: torch.Tensor, k_codes: torch.Tensor, k_scales:
         _require(t.is_contiguous(), f"{name} must be contiguous")
     _require(q.dim() == 3 and k_tree.dim() == 3 and k_codes.dim() == 3,
              "q/k_tree must be [R, H, D] and k_codes [Hkv, tokens, D/2]")
-    rows, hq, dim = q.shape
-    hkv = k_codes.shape[0]
     _require(k_codes.shape == v_codes.shape and k_codes.stride() == v_codes.stride()
              and k_scales.stride() == v_scales.stride(),
              "k and v codes and scales must share shape and strides")
-    _require(k_codes.shape[2] * 2 == dim, "head dims disagree")
+    _require(k_codes.shape[2] * 2 == q.shape[2], "head dims disagree")
     _require(not any((t.data_ptr() | t.stride(0) | t.stride(1)) % 16 for t in (k_codes, v_codes)),
              "codes must be 16-byte aligned, their strides multiples of 16 bytes")
-    _require(k_tree.shape == (rows, hkv, dim) and v_tree.shape == k_tree.shape
-             and k_tree.stride() == v_tree.stride(),
+    _require(k_tree.shape == (q.shape[0], k_codes.shape[0], q.shape[2])
+             and v_tree.shape == k_tree.shape and k_tree.stride() == v_tree.stride(),
              "k_tree/v_tree must be [R, Hkv, D] with equal strides")
-    n = prefix_len.numel()
-    check_plan_call(plan, n, rows, hq, hkv, dim)
     _require(plan.device is not None and plan.device.is_cuda, "plan is not on the device")
-    _require(parent.numel() >= rows, "parent must cover every packed row")
-    _require(row_offset.numel() == n + 1 and prefix_start.numel() == n,
+    _require(parent.numel() >= q.shape[0], "parent must cover every packed row")
+    _require(row_offset.numel() == prefix_len.numel() + 1
+             and prefix_start.numel() == prefix_len.numel(),
              "request metadata sizes disagree")
     if status is not None:
         _check_device_tensor(status, "status", torch.int32)
-    if out is None:
-        out = torch.empty((rows, hq, dim), dtype=torch.bfloat16, device=q.device)
-    _check_rows(out, "out")
-    _require(out.shape == (rows, hq, dim), "out must be [R, Hq, D]")
+    if out is not None:
+        _check_rows(out, "out")
+        _require(out.shape == q.shape, "out must be [R, Hq, D]")
+    for t, name in ((k_codes, "k_codes"), (k_scales, "k_scales"), (v_codes, "v_codes"),
+                    (v_scales, "v_scales"), (k_tree, "k_tree"), (v_tree, "v_tree"),
+                    (row_offset, "row_offset"), (prefix_start, "prefix_start"),
+                    (prefix_len, "prefix_len"), (parent, "parent"), (out, "out"),
+                    (status, "status"), (plan.device, "plan")):
+        _require(t is None or t.device == q.device, f"{name} must be on q's device")
     _check_current(q, "q")
+
+
+def _mx4_attention_args(q, k_codes, k_scales, v_codes, v_scales, k_tree, v_tree, row_offset,
+                        prefix_start, prefix_len, parent, plan, out, scale, status):
+    """The call's argument struct and output, of arguments that fit.
+
+    A call takes a few microseconds on the GPU at the least, so everything is
+    looked at once here; what is wrong is found out by _explain_mx4_attention."""
+    try:
+        bf16, u8, i32 = torch.bfloat16, torch.uint8, torch.int32
+        rows, hq, dim = q.shape
+        hkv, tokens, half = k_codes.shape
+        qs, cs, ss, ts = q.stride(), k_codes.stride(), k_scales.stride(), k_tree.stride()
+        at = (q.data_ptr(), k_codes.data_ptr(), v_codes.data_ptr(), k_tree.data_ptr(),
+              v_tree.data_ptr())
+        n = prefix_len.numel()
+        device = q.get_device()  # -1 on the CPU
+        kv = (hkv, tokens, half // 16)
+        fits = (
+            q.dtype == bf16 and k_tree.dtype == bf16 and v_tree.dtype == bf16
+            and k_codes.dtype == u8 and k_scales.dtype == u8 and v_codes.dtype == u8
+            and v_scales.dtype == u8 and row_offset.dtype == i32 and prefix_len.dtype == i32
+            and parent.dtype == i32 and prefix_start.dtype == torch.int64
+            and 2 * half == dim and v_codes.shape == k_codes.shape
+            and v_scales.shape == kv and k_scales.shape == kv
+            and k_tree.shape == (rows, hkv, dim) and v_tree.shape == k_tree.shape
+            and v_codes.stride() == cs and v_scales.stride() == ss and v_tree.stride() == ts
+            and qs[2] == 1 and cs[2] == 1 and (ss[2] == 1 or half == 16) and ts[2] == 1
+            and not (at[0] | at[1] | at[2] | at[3] | at[4] | cs[0] | cs[1]) & 15
+            and not (qs[0] | qs[1] | ts[0] | ts[1]) & 7
+            and row_offset.numel() == n + 1 and prefix_start.numel() == n
+            and parent.numel() >= rows and row_offset.is_contiguous()
+            and prefix_len.is_contiguous() and parent.is_contiguous()
+            and prefix_start.is_contiguous()
+            and device == torch.cuda.current_device()
+            and k_codes.get_device() == device and k_scales.get_device() == device
+            and v_codes.get_device() == device and v_scales.get_device() == device
+            and k_tree.get_device() == device and v_tree.get_device() == device
+            and row_offset.get_device() == device and prefix_len.get_device() == device
+            and parent.get_device() == device and prefix_start.get_device() == device
+            and plan.device is not None and plan.device.get_device() == device)
+    except (AttributeError, TypeError, ValueError, RuntimeError):  # no tensors, no GPU
+        fits = False
+    if not fits or out is not None or status is not None:
+        _explain_mx4_attention(q, k_codes, k_scales, v_codes, v_scales, k_tree, v_tree,
+                               row_offset, prefix_start, prefix_len, parent, plan, out, status)
+    _require(fits, "the arguments do not fit together")
+    check_plan_call(plan, n, rows, hq, hkv, dim)
+    if out is None:
+        out = torch.empty((rows, hq, dim), dtype=bf16, device=q.device)
+    os = out.stride()
     workspace = plan.workspace
     attn = _lib.SgTreeAttnArgs(
         n, rows, hq, hkv, dim, float(dim ** -0.5 if scale is None else scale),
-        q.data_ptr(), q.stride(0), q.stride(1),
-        k_codes.data_ptr(), v_codes.data_ptr(), k_codes.stride(0), k_codes.stride(1),
-        k_tree.data_ptr(), v_tree.data_ptr(), k_tree.stride(0), k_tree.stride(1),
+        at[0], qs[0], qs[1], at[1], at[2], cs[0], cs[1], at[3], at[4], ts[0], ts[1],
         row_offset.data_ptr(), prefix_start.data_ptr(), prefix_len.data_ptr(),
-        parent.data_ptr(), out.data_ptr(), out.stride(0), out.stride(1),
+        parent.data_ptr(), out.data_ptr(), os[0], os[1],
         plan.device.data_ptr(), plan.host.ctypes.data, plan.units, plan.merges,
         workspace.data_ptr() if workspace is not None else 0,
         workspace.numel() if workspace is not None else 0,
         status.data_ptr() if status is not None else 0)
-    a = _lib.SgTreeAttnMx4Args(attn, k_scales.data_ptr(), v_scales.data_ptr(),
-                               k_scales.stride(0), k_scales.stride(1))
-    keep = (q, k_codes, k_scales, v_codes, v_scales, k_tree, v_tree, row_offset, prefix_start,
-            prefix_len, parent, plan, out, status)
-    return PreparedCall("sg_tree_attn_mx4_fwd", a, keep, result=out)
+    return _lib.SgTreeAttnMx4Args(attn, k_scales.data_ptr(), v_scales.data_ptr(), ss[0],
+                                  ss[1]), out
 
 
 def kv_commit_mx4(k_code_ptrs: torch.Tensor, k_scale_ptrs: torch.Tensor,
@@ -1053,16 +1115,17 @@ class Fp8Rows:
 
 
 def _new_fp8_rows(rows: int, columns: int, device) -> "tuple[Fp8Rows, _lib.SgFp8RowsOut]":
-    padded = (columns + FP8_BLOCK - 1) // FP8_BLOCK * FP8_BLOCK
+    blocks = (columns + FP8_BLOCK - 1) // FP8_BLOCK
+    padded = blocks * FP8_BLOCK
     codes = torch.empty((rows, padded), dtype=torch.float8_e4m3fn, device=device)
-    scales = torch.empty((padded // FP8_BLOCK, rows), dtype=torch.float32, device=device)
+    scales = torch.empty_strided((rows, blocks), (1, rows), dtype=torch.float32, device=device)
     out = _lib.SgFp8RowsOut(codes.data_ptr(), padded, scales.data_ptr(), rows)
-    return Fp8Rows(codes[:, :columns], scales.T), out
+    return Fp8Rows(codes if padded == columns else codes[:, :columns], scales), out
 
 
 def _check_current(t: torch.Tensor, name: str) -> None:
-    _require(t.device.index == torch.cuda.current_device(),
-             f"{name} is on {t.device}, which is not the current device")
+    if t.get_device() != torch.cuda.current_device():
+        raise ValueError(f"{name} is on {t.device}, which is not the current device")
 
 
 def quantize_fp8(x: torch.Tensor) -> Fp8Rows:
@@ -1071,8 +1134,9 @@ def quantize_fp8(x: torch.Tensor) -> Fp8Rows:
     _check_rows(x, "x")
     _require(x.dim() == 2, "x must be [R, K]")
     _check_current(x, "x")
-    rows, out = _new_fp8_rows(x.shape[0], x.shape[1], x.device)
-    _lib.check(_lib.load().sg_fp8_quantize_rows(x.data_ptr(), x.stride(0), x.shape[0], x.shape[1],
+    count, columns = x.shape
+    rows, out = _new_fp8_rows(count, columns, x.device)
+    _lib.check(_lib.load().sg_fp8_quantize_rows(x.data_ptr(), x.stride(0), count, columns,
                                                 ctypes.byref(out), _stream_handle()),
                "sg_fp8_quantize_rows")
     return rows
@@ -1139,33 +1203,35 @@ def fp8_matmul(rows: Fp8Rows, weight: PackedFp8Weight,
     _check_device_tensor(codes, "codes", torch.float8_e4m3fn)
     _check_device_tensor(scales, "scales", torch.float32)
     n, k = weight.shape
-    count = codes.shape[0]
-    blocks = -(-k // FP8_BLOCK)
+    blocks = (k + FP8_BLOCK - 1) // FP8_BLOCK
     _require(codes.dim() == 2 and codes.shape[1] == k, "rows and weight disagree on K")
-    _require(tuple(scales.shape) == (count, blocks) and (scales.stride(0) == 1 or count == 1),
+    count = codes.shape[0]
+    device = codes.device
+    cs, ss = codes.stride(), scales.stride()
+    _require(scales.shape == (count, blocks) and (ss[0] == 1 or count == 1),
              "scales must be the [R, ceil(K/128)] view of the quantized rows")
-    _require(codes.device == weight.device and scales.device == codes.device,
+    _require(codes.get_device() == weight.packed.get_device() == scales.get_device(),
              "rows and weight must be on one device")
     _check_current(codes, "rows")
     # The padded columns behind a row are read: they must be there.
-    behind = codes.untyped_storage().nbytes() - codes.storage_offset()
-    _require(count == 0 or (codes.stride(1) == 1 and codes.stride(0) >= FP8_BLOCK * blocks
-                            and behind >= (count - 1) * codes.stride(0) + FP8_BLOCK * blocks),
+    _require(count == 0 or (cs[1] == 1 and cs[0] >= FP8_BLOCK * blocks
+                            and codes.untyped_storage().nbytes() - codes.storage_offset()
+                            >= (count - 1) * cs[0] + FP8_BLOCK * blocks),
              "codes must be rows padded with zeros to 128 columns")
     if out is None:
-        out = torch.empty((count, (n + 7) // 8 * 8), dtype=torch.bfloat16,
-                          device=codes.device)[:, :n]
+        out = torch.empty((count, (n + 7) // 8 * 8), dtype=torch.bfloat16, device=device)
+        if n % 8:
+            out = out[:, :n]
     else:
         _check_rows(out, "out")
-        _require(tuple(out.shape) == (count, n) and out.device == codes.device,
+        _require(tuple(out.shape) == (count, n) and out.device == device,
                  "out must be [R, N] on the rows' device")
     lib = _lib.load()
-    nbytes = int(lib.sg_fp8_matmul_workspace_bytes(count, n, k))
-    workspace = (torch.empty(nbytes, dtype=torch.uint8, device=codes.device)
-                 if nbytes > 0 else None)
+    nbytes = lib.sg_fp8_matmul_workspace_bytes(count, n, k)
+    workspace = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes > 0 else None
     a = _lib.SgFp8MatmulArgs(
-        count, n, k, 0, codes.data_ptr(), codes.stride(0), scales.data_ptr(),
-        scales.stride(1) if blocks > 1 else max(count, 1), weight.packed.data_ptr(),
+        count, n, k, 0, codes.data_ptr(), cs[0], scales.data_ptr(),
+        ss[1] if blocks > 1 else max(count, 1), weight.packed.data_ptr(),
         weight.scales.data_ptr(), out.data_ptr(), out.stride(0),
         workspace.data_ptr() if workspace is not None else 0, max(nbytes, 0))
     _lib.check(lib.sg_fp8_matmul(ctypes.byref(a), _stream_handle()), "sg_fp8_matmul")

@@ -101,21 +101,19 @@ def add_rmsnorm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float,
     ops._require(x.dim() == 2, "x must be [R, H]")
     rows, hidden = x.shape
     ops._check_rows(weight, "weight")
-    ops._require(tuple(weight.shape) == (hidden,), "weight must be [H]")
+    ops._require(weight.shape == (hidden,), "weight must be [H]")
     if residual is not None:
         ops._check_rows(residual, "residual")
         ops._require(residual.shape == x.shape, "residual must be [R, H]")
     ops._check_current(x, "x")
     normed, out = ops._new_fp8_rows(rows, hidden, x.device)
     total = (torch.empty((rows, hidden), dtype=x.dtype, device=x.device) if want_sum else None)
-    a = _lib.SgAddRmsNormArgs()
-    a.num_rows, a.hidden, a.eps = rows, hidden, float(eps)
-    a.x_dev, a.x_stride = x.data_ptr(), x.stride(0)
-    if residual is not None:
-        a.residual_dev, a.residual_stride = residual.data_ptr(), residual.stride(0)
-    a.weight_dev = weight.data_ptr()
-    if total is not None:
-        a.residual_out_dev, a.residual_out_stride = total.data_ptr(), total.stride(0)
+    # Positional, in the order of SgAddRmsNormArgs' fields.
+    a = _lib.SgAddRmsNormArgs(
+        rows, hidden, float(eps), 0, x.data_ptr(), x.stride(0),
+        residual.data_ptr() if residual is not None else 0,
+        residual.stride(0) if residual is not None else 0, weight.data_ptr(), 0, 0,
+        total.data_ptr() if total is not None else 0, hidden if total is not None else 0)
     _lib.check(_lib.load().sg_add_rmsnorm_fp8(ctypes.byref(a), ctypes.byref(out), _stream()),
                "sg_add_rmsnorm_fp8")
     return (normed, total) if want_sum else normed
