@@ -7,16 +7,30 @@
 // prefix's values are bf16 values, so the products are the bf16 kernel's over
 // the unpacked cache.
 //
-// A window is 64 keys.  Its codes are 9.2 KB (32 KB in bf16): too few bytes to
-// keep in LDS as copies in flight, so every thread loads one 16-byte piece of K
-// and one of V (32 values, one scale) into registers two windows ahead, unpacks
-// them to bf16 (gfx950: two values an instruction, scale included) and writes
-// them to the LDS stage that the previous window finished reading.  One barrier
-// a window.  Unpacked once for the workgroup: 32 conversions a thread and
-// window, where every wave for itself would need 128.
-//   S^T = K Q^T and O^T += V^T P^T with v_mfma_f32_32x32x16_bf16, softmax in
-//   registers, one query column per lane pair, as in tree_attn.hip.
-// The wave's own (bf16) rows come first, while the first windows are loaded.
+// K is multiplied as it is held: v_mfma_scale_f32_32x32x64_f8f6f4 takes e2m1
+// elements with a power-of-two scale for 32 of them, so S^T = K Q^T needs no
+// unpacking and no LDS, if Q is in 8 bits.  A bf16 value's 8 significant bits are
+// the sum of two e4m3 values of 4 each, q = hi + lo exactly, with a scale for 32
+// columns (a value below 2^-14 of its block's largest keeps fewer bits, an error
+// below 2^-22 of that); two products each, in the time of the bf16 ones.
+// V is unpacked to bf16 (gfx950: two values an instruction, scale included) into
+// LDS and read transposed (ds_read_b64_tr_b16) for O^T += V^T P^T with
+// v_mfma_f32_32x32x16_bf16, as in tree_attn.hip.
+//
+// Waves.  A wave takes one q-group of 32 query vectors over 32-key tiles; 1 q-group:
+// four key streams, each wave with V tiles of its own and no barrier; 2: two
+// streams; 3-4: one.  There the workgroup unpacks 64 keys of V at a time together,
+// a piece a thread, into one of two stages (one barrier for 64 keys).  Codes are
+// loaded two tiles (stages) ahead into registers: a tile is 4.3 KB.  Two workgroups
+// share a CU; streams are merged at the end.
+//
+// Measured (64 requests of 16,384 cached tokens, 32 q / 8 kv heads, d = 128; 1 / 16 /
+// 32 rows each): 243 / 432 / 644 us, that is 4.7 / 2.6 / 1.8 TB/s of codes and scales
+// and 71 / 636 / 854 TFLOP/s.  One row a request is bound by the cache's bytes, 32
+// by issue: a wave and tile take 124 vector instructions and 20 products.  Tried:
+// K and V unpacked to bf16 by the workgroup, 406 / 444 / 702; by each wave for
+// itself, 249 / 470 / 873; the products of a tile issued before the softmax of the
+// one before it, 583 / 381 / 672 (spills at one row).
 #include <type_traits>
 
 #include "tree_attn_common.h"
@@ -24,8 +38,25 @@
 namespace sg {
 namespace {
 
-constexpr int kWindow = 64;  // keys of a window: two 32-key blocks
 constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / 64;
+
+typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+typedef __attribute__((ext_vector_type(2))) short short2_t;
+typedef __attribute__((ext_vector_type(8))) int intx8;
+
+__device__ __forceinline__ bf16x2 as_pair(uint32_t w) { return __builtin_bit_cast(bf16x2, w); }
+
+// XOR swizzle of the 16-byte chunks of V's LDS row r.  The transposed reads take 64
+// bytes of each of four consecutive rows: bits 2 and 3 (bit 2 at D = 64, where two
+// rows fill the banks) put those on different banks.  The unpacked writes take one
+// chunk of each block of four (two) consecutive rows: the low bits.  (4 (r & 3) +
+// 2 (r >> 1 & 1), right for the reads alone, spent half of the LDS's active cycles
+// on conflicts of the writes.)  Both repeat every four rows.
+template <int D>
+__host__ __device__ constexpr int swz_w(int r) {
+  return D == 128 ? 5 * (r & 3) : 5 * ((r >> 1) & 1);
+}
 
 // 16-byte chunk c (8 values) of 32 unpacked ones, from code word `w` of a block.
 __device__ __forceinline__ uint4 unpack8(uint32_t w, float scale) {
@@ -45,46 +76,55 @@ __device__ __forceinline__ uint32_t nonfinite_halves(uint32_t w) {
   return lo | hi;
 }
 
-// LDS of a workgroup: two stages of K and two of V (the merge scratch and the
-// output staging after the last window), and the tree's tables.
+// The call's arguments where the launch put them.  What is read through a fresh()
+// pointer is loaded there and then: kept in registers from the kernel's start,
+// the arguments filled the scalar ones, and every load of the loop moved 30 of
+// their words back from vector lanes first.
+using ArgsIn = const __attribute__((address_space(4))) SgTreeAttnMx4Args*;
+__device__ __forceinline__ ArgsIn fresh(ArgsIn p) {
+  asm volatile("" : "+s"(p));
+  return p;
+}
+// A scalar address that is not put together again from its parts at every use.
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+using GlobalBytes = const __attribute__((address_space(1))) unsigned char*;
+using GlobalU4 = const __attribute__((address_space(1))) u32x4*;
+__device__ __forceinline__ GlobalBytes settled(const unsigned char* p) {
+  GlobalBytes g = (GlobalBytes)p;
+  asm volatile("" : "+s"(g));
+  return g;
+}
+
+// LDS of a workgroup: 8 KB of V (D = 128) a wave, after the last tile the merge
+// scratch and the output staging; and the tree's tables.
 template <int D>
 struct Shared {
-  __align__(1024) unsigned char ring[4 * 2 * kTileKeys * D * 2];
+  static constexpr int kSlot = (2 + D / 2) * 64 * 4;   // a wave's state
+  static constexpr int kStage = 32 * (2 * D + 16);     // a wave's output rows
+  static constexpr int kBytes = (kWaves - 1) * kSlot + kStage;
+  static_assert(kBytes >= kWaves * kTileKeys * 2 * D && kBytes >= kSlot * 2 + kStage * 2 &&
+                    kBytes >= kStage * 4,
+                "every use of the buffer must fit");
+  __align__(1024) unsigned char buf[kBytes];
   uint32_t anc[kQPerUnit][kAncWords];
   int2 run[kMaxTreeRows];
-  uint32_t odd[kAncWords];  // blocks of 32 tree rows with a V that is no number
 };
 
-// One unit.  kTwo: of 1-2 q-groups; two waves share one and take a 32-key block of
-// each window (key streams, merged at the end).  Otherwise (3-4) a wave takes
-// both blocks.
-template <int D, bool kTwo>
-__device__ __forceinline__ void attn_unit_mx4(const SgTreeAttnMx4Args& args, const AttnUnit& u,
-                                              Shared<D>& sh) {
+// One unit.  kShared: of 2-4 q-groups, V unpacked by the workgroup; kBoth: of 3-4, a
+// wave takes both tiles of a stage.
+template <int D, bool kShared, bool kBoth>
+__device__ __forceinline__ void attn_unit_mx4(const SgTreeAttnMx4Args& args, ArgsIn in,
+                                              const AttnUnit& u, Shared<D>& sh) {
   const SgTreeAttnArgs& a = args.attn;
-  constexpr int KB = D / 16;                  // QK^T k-blocks of 16 head dims
-  constexpr int DB = D / 32;                  // PV blocks of 32 head dims
+  constexpr int KB = D / 16;                  // QK^T products of 16 columns
+  constexpr int DB = D / 32;                  // PV blocks of 32 columns
   constexpr int ROWB = D * 2;                 // bytes of an LDS row
-  constexpr int TILEB = kTileKeys * ROWB;     // bytes of 32 keys of K (or V)
-  constexpr int STAGEB = 2 * TILEB;           // bytes of a window of K (or V)
-  constexpr int LOADS = D / 64;               // pieces a thread moves per window
-  constexpr int STATE = 2 + 16 * DB;          // floats per lane of a WaveState
-  constexpr int kSlotBytes = STATE * 64 * 4;
-  constexpr int kRowBytes = 2 * D;
-  constexpr int kPitch = kRowBytes + 16;
-  static_assert(2 * kSlotBytes + 2 * 32 * kPitch <= 4 * STAGEB &&
-                    4 * 32 * kPitch <= 4 * STAGEB,
-                "merge scratch and output staging must fit the ring");
-  unsigned char* const s_ring = sh.ring;
-  uint32_t(*const s_anc)[kAncWords] = sh.anc;
-  uint32_t* const s_odd = sh.odd;
-  unsigned char* const s_k = s_ring;
-  unsigned char* const s_v = s_ring + 2 * STAGEB;
+  constexpr int P = D / 64;                   // 16-byte pieces of codes a lane loads of K (and V)
+  constexpr int kPitch = ROWB + 16;
 
   const int G = a.num_q_heads / a.num_kv_heads;
   // Opaque, so that what follows from it is not kept in registers from one unit
-  // of a list to the next (83 registers spilled, and a spill's reload waits for
-  // the loads in flight).
+  // of a list to the next.
   int tid = threadIdx.x;
   asm volatile("" : "+v"(tid));
   const int lane = tid & 63;
@@ -101,8 +141,8 @@ __device__ __forceinline__ void attn_unit_mx4(const SgTreeAttnMx4Args& args, con
     poison_unit<D>(a, u, r0);
     return;
   }
-  const int nq = (u.row_count * G + 31) / 32;
-  constexpr int streams = kTwo ? 2 : 1;
+  const int nq = (u.row_count * G + 31) / 32;   // q-groups in use, 1..4
+  constexpr int streams = kBoth ? 1 : kShared ? 2 : 4;  // key streams of each
   const int qg = wave % nq;
   const int ks = wave / nq;
   const bool active = ks < streams;
@@ -114,102 +154,169 @@ __device__ __forceinline__ void attn_unit_mx4(const SgTreeAttnMx4Args& args, con
   const int g = u.kv_head;
   const bool do_tree = (u.flags & 1) != 0;
 
-  // Pieces of this thread: key row and 32-value block of the window, K or V.
-  // A window's base is scalar, a piece's offset one register for K and V.
-  constexpr int kBlocks = D / 32;             // 32-value blocks of a row
+  // Codes and scales of this lane.  K: of key pi(col) of a tile, piece j holds
+  // columns 64 j + 32 half .. +31, an operand of product j.  V: piece i is 32
+  // columns of a row, of a tile or (shared) of a window's 64 keys.
   const int prefix_keys = u.key_end - u.key_begin;
-  const int windows = (prefix_keys + kWindow - 1) / kWindow;
-  const int full = prefix_keys / kWindow;
+  const int tiles = active ? (prefix_keys + kTileKeys - 1) / kTileKeys : 0;
   const int64_t prefix0 = a.prefix_start_dev[u.req] + u.key_begin;
   const int64_t code0 = g * a.cache_head_stride + prefix0 * a.cache_token_stride;
   const int64_t scale0 = g * args.scale_head_stride + prefix0 * args.scale_token_stride;
-  const int piece = D == 128 ? tid : tid & 127;
-  const int p_row = piece / kBlocks;
-  const int p_blk = piece % kBlocks;
-  const bool v_wave = wave >= kThreads / 128;  // D = 64: the upper waves move V
-  const uint32_t c_lane = p_row * static_cast<uint32_t>(a.cache_token_stride) + 16 * p_blk;
-  const uint32_t s_lane = p_row * static_cast<uint32_t>(args.scale_token_stride) + p_blk;
+  const GlobalBytes k_codes =
+      settled(static_cast<const unsigned char*>(a.k_cache_dev) + code0);
+  const GlobalBytes v_codes =
+      settled(static_cast<const unsigned char*>(a.v_cache_dev) + code0);
+  const GlobalBytes k_scales =
+      settled(static_cast<const unsigned char*>(args.k_scale_dev) + scale0);
+  const GlobalBytes v_scales =
+      settled(static_cast<const unsigned char*>(args.v_scale_dev) + scale0);
+  uint32_t c_stride = static_cast<uint32_t>(a.cache_token_stride);
+  uint32_t s_stride = static_cast<uint32_t>(args.scale_token_stride);
+  asm volatile("" : "+s"(c_stride), "+s"(s_stride));
+  const int k_key = key_pi(col);
+  constexpr int kBlocks = D / 32;             // 32-column blocks of a row
+  const int v_row = lane / kBlocks;           // of piece 0; piece i: + 64 / kBlocks
+  const int v_blk = lane % kBlocks;
+  constexpr int kVStep = 64 / kBlocks;
+  constexpr int kWindow = 2 * kTileKeys;      // keys of a shared stage
+  const int w_row = tid / kBlocks;            // of a window's piece, below kWindow
+  const bool w_piece = kWindow * kBlocks >= kThreads || wave < kWindow * kBlocks / 64;
   struct Raw {
-    uint4 code[LOADS];
-    uint32_t scale[LOADS];
+    u32x4 c[P];
+    uint32_t s[P];
   };
-  // Window w of the prefix into registers.  Keys past the range read the last
-  // valid one: its score is masked, its probability 0.
-  auto load = [&](int w, Raw& r) {
-    uint32_t c_off = c_lane, s_off = s_lane;
-    if (w >= full) {
-      const int key = min(p_row, prefix_keys - 1 - w * kWindow);
-      c_off = key * static_cast<uint32_t>(a.cache_token_stride) + 16 * p_blk;
-      s_off = key * static_cast<uint32_t>(args.scale_token_stride) + p_blk;
+  // Offsets inside a whole tile (window).
+  const uint32_t kc_at = k_key * c_stride + 16 * half, ks_at = k_key * s_stride + half;
+  uint32_t vc_at[P], vs_at[P];
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    vc_at[i] = (kShared ? w_row : v_row + kVStep * i) * c_stride + 16 * v_blk;
+    vs_at[i] = (kShared ? w_row : v_row + kVStep * i) * s_stride + v_blk;
+  }
+  // Keys past the range read the last valid one: its score is masked, its
+  // probability 0.
+  auto load_k = [&](int t, Raw& r) {
+    const GlobalBytes c = k_codes + static_cast<int64_t>(t) * kTileKeys * c_stride;
+    const GlobalBytes s = k_scales + static_cast<int64_t>(t) * kTileKeys * s_stride;
+    uint32_t ca = kc_at, sa = ks_at;
+    const int last = prefix_keys - 1 - t * kTileKeys;
+    if (last < kTileKeys - 1) {
+      const uint32_t key = min(k_key, last);
+      ca = key * c_stride + 16 * half;
+      sa = key * s_stride + half;
     }
-    const int64_t cb = code0 + static_cast<int64_t>(w) * kWindow * a.cache_token_stride;
-    const int64_t sb = scale0 + static_cast<int64_t>(w) * kWindow * args.scale_token_stride;
 #pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-      const bool is_v = D == 128 ? i == 1 : v_wave;
-      const unsigned char* c =
-          static_cast<const unsigned char*>(is_v ? a.v_cache_dev : a.k_cache_dev) + cb;
-      const unsigned char* b =
-          static_cast<const unsigned char*>(is_v ? args.v_scale_dev : args.k_scale_dev) + sb;
-      r.code[i] = *reinterpret_cast<const uint4*>(c + c_off);
-      r.scale[i] = b[s_off];
-    }
-  };
-  // LDS offsets of the piece's first 16-byte chunk (of four) in stage 0 of K and
-  // V.  The swizzles are XORs of the chunk index, so chunk c is at that ^ 16 c.
-  const int k_row = (p_row & 32) + key_slot(p_row & 31);
-  const uint32_t k_at = k_row * ROWB + 16 * ((4 * p_blk) ^ swz_k<D>(k_row));
-  const uint32_t v_at = p_row * ROWB + 16 * ((4 * p_blk) ^ swz_v<D>(p_row));
-  const uint32_t one_at = v_wave ? v_at + 2 * STAGEB : k_at;  // D = 64
-  auto piece_at = [&](int i, int c) {
-    return s_ring + (D == 128 ? (i == 1 ? (v_at ^ (16 * c)) + 2 * STAGEB : k_at ^ (16 * c))
-                              : one_at ^ (16 * c));
-  };
-  auto unpack = [&](const Raw& r, int stage) {
-#pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-      const float s = __uint_as_float(r.scale[i] << 23);  // 255: converts to NaN
-      const uint32_t w[4] = {r.code[i].x, r.code[i].y, r.code[i].z, r.code[i].w};
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-        *reinterpret_cast<uint4*>(piece_at(i, c) + stage * STAGEB) = unpack8(w[c], s);
+    for (int j = 0; j < P; ++j) {
+      r.c[j] = *(GlobalU4)(c + ca + 32 * j);
+      r.s[j] = s[sa + 2 * j];
     }
   };
-  // raw[p] holds window w with w & 1 == p.
-  Raw raw[2];
-  if (windows > 0) load(0, raw[0]);
-  if (windows > 1) load(1, raw[1]);
-
-  if (tid < kAncWords) s_odd[tid] = 0u;  // published by the barriers of what follows
-  if (do_tree) build_ancestors(a, u, r0, n, sh.run, s_anc);
-
-  // Query operand: lane supplies Q[row, head, 16*kb + 8*half .. +7].
-  bf16x8 qf[KB];
-  {
-    const uint16_t* qp = static_cast<const uint16_t*>(a.q_dev) + row * a.q_row_stride +
-                         static_cast<int64_t>(head) * a.q_head_stride + 8 * half;
+  // Tile t's V (private), window t's piece of this thread (shared).
+  auto load_v = [&](int t, Raw& r) {
+    constexpr int kKeys = kShared ? kWindow : kTileKeys;
+    if (kShared && !w_piece) return;
+    const GlobalBytes c = v_codes + static_cast<int64_t>(t) * kKeys * c_stride;
+    const GlobalBytes s = v_scales + static_cast<int64_t>(t) * kKeys * s_stride;
+    const int last = prefix_keys - 1 - t * kKeys;
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb)
-      qf[kb] = as_bf16x8(q_valid ? *reinterpret_cast<const uint4*>(qp + 16 * kb) : zero4());
+    for (int i = 0; i < (kShared ? 1 : P); ++i) {
+      uint32_t ca = vc_at[i], sa = vs_at[i];
+      if (last < kKeys - 1) {
+        const uint32_t key = min(kShared ? w_row : v_row + kVStep * i, last);
+        ca = key * c_stride + 16 * v_blk;
+        sa = key * s_stride + v_blk;
+      }
+      r.c[i] = *(GlobalU4)(c + ca);
+      r.s[i] = s[sa];
+    }
+  };
+  // rk[p], rv[p]: this wave's tiles (windows) of even (odd) number.
+  const int windows = (prefix_keys + kWindow - 1) / kWindow;
+  Raw rk[2], rv[2];
+  if (ks < tiles) load_k(ks, rk[0]);
+  if (!kBoth && ks + streams < tiles) load_k(ks + streams, rk[1]);
+  if constexpr (kShared) {
+    if (windows > 0) load_v(0, rv[0]);
+    if (windows > 1) load_v(1, rv[1]);
+  } else {
+    if (ks < tiles) load_v(ks, rv[0]);
+    if (ks + streams < tiles) load_v(ks + streams, rv[1]);
   }
 
-  // LDS read addresses of this lane inside a 32-key block.
+  if (do_tree) build_ancestors(a, u, r0, n, sh.run, sh.anc);
+
+  // The query vector in two 8-bit terms.  Product j takes columns 64 j .. +63: this
+  // lane's bytes 0-15 are columns 64 j + 16 half .. +15, bytes 16-31 those 32 on;
+  // the scale of block b (32 columns) is read from lane half b.
+  const uint16_t* const q_row = static_cast<const uint16_t*>(a.q_dev) + row * a.q_row_stride +
+                                static_cast<int64_t>(head) * a.q_head_stride;
+  intx8 q_hi[P], q_lo[P];
+  int q_scale[P];  // bytes 0, 1: of hi and lo
+#pragma unroll
+  for (int j = 0; j < P; ++j) {
+    int code[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      uint32_t w[8];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const uint4 v = q_valid ? *reinterpret_cast<const uint4*>(q_row + 64 * j + 32 * b +
+                                                                  16 * half + 8 * e)
+                                : zero4();
+        w[4 * e] = v.x, w[4 * e + 1] = v.y, w[4 * e + 2] = v.z, w[4 * e + 3] = v.w;
+      }
+      uint32_t most = 0u;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) most = max(max(most, (w[e] << 16) & 0x7fffffffu),
+                                             w[e] & 0x7fff0000u);
+      const auto both = __builtin_amdgcn_permlane32_swap(most, most, false, false);
+      const int top = static_cast<int>(max(both[0], both[1]) >> 23);
+      code[b] = min(max(top - 7, 5), 254);  // the largest magnitude is below 256
+      const float x_hi = __uint_as_float(static_cast<uint32_t>(code[b]) << 23);
+      const float x_lo = __uint_as_float(static_cast<uint32_t>(code[b] - 4) << 23);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        short2_t hi = {0, 0}, lo = {0, 0};
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const uint32_t whole = w[2 * e + k], head4 = whole & 0xfff0fff0u;
+          const float lo0 = __uint_as_float(whole << 16) - __uint_as_float(head4 << 16);
+          const float lo1 =
+              __uint_as_float(whole & 0xffff0000u) - __uint_as_float(head4 & 0xffff0000u);
+          if (k == 0) {
+            hi = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(hi, as_pair(head4), x_hi, false);
+            lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(lo, lo0, lo1, x_lo, false);
+          } else {
+            hi = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(hi, as_pair(head4), x_hi, true);
+            lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(lo, lo0, lo1, x_lo, true);
+          }
+        }
+        // An infinity or a NaN: the block is NaN.
+        q_hi[j][4 * b + e] = top == 255 ? 0x7f7f7f7f : __builtin_bit_cast(int, hi);
+        q_lo[j][4 * b + e] = __builtin_bit_cast(int, lo);
+      }
+    }
+    q_scale[j] = half == 0 ? code[0] | (code[0] - 4) << 8 : code[1] | (code[1] - 4) << 8;
+  }
+
+  // LDS of this wave's V tile.  Chunk c of row r is at c ^ swz(r): a block's chunk c
+  // is at its first one's address ^ 16 c.
+  unsigned char* const s_v = sh.buf + wave * kTileKeys * ROWB;
+  uint32_t v_at[P];
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    const int r = v_row + kVStep * i;
+    v_at[i] = r * ROWB + 16 * ((4 * v_blk) ^ swz_w<D>(r));
+  }
   const int gq = lane >> 4;
   const int jj = lane & 15;
   const int rr = jj >> 2;
   const int cc = jj & 3;
-  int k_off[KB];
-#pragma unroll
-  for (int kb = 0; kb < KB; ++kb) k_off[kb] = col * ROWB + 16 * ((2 * kb + half) ^ swz_k<D>(col));
-  int v_off[DB][2];
-#pragma unroll
-  for (int db = 0; db < DB; ++db)
-#pragma unroll
-    for (int hi = 0; hi < 2; ++hi) {
-      const int vrow = 16 * half + 4 * hi + rr;
-      const int chunk = 4 * db + 2 * (gq & 1) + (cc >> 1);
-      v_off[db][hi] = vrow * ROWB + 16 * (chunk ^ swz_v<D>(vrow)) + 8 * (cc & 1);
-    }
+  // Of the transposed reads: column block db is at v_read ^ 64 db, and the rows 4 on
+  // have the same swizzle.
+  const int v_first = 16 * half + rr;
+  const int v_read = v_first * ROWB +
+                     16 * ((2 * (gq & 1) + (cc >> 1)) ^ swz_w<D>(v_first)) + 8 * (cc & 1);
 
   const float c2 = a.scale * kLog2e;
   WaveState<D> st;
@@ -220,21 +327,47 @@ __device__ __forceinline__ void attn_unit_mx4(const SgTreeAttnMx4Args& args, con
 #pragma unroll
     for (int r = 0; r < 16; ++r) st.acc[db][r] = 0.0f;
 
-  // S^T of the 32-key block at LDS byte `at` of the K stages.
-  auto qk = [&](int at) {
+  auto qk = [&](const Raw& r) {
     floatx16 s;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] = 0.0f;
+    for (int e = 0; e < 16; ++e) s[e] = 0.0f;
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb)
-      s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-          as_bf16x8(*reinterpret_cast<const uint4*>(s_k + at + k_off[kb])), qf[kb], s, 0, 0, 0);
+    for (int j = 0; j < P; ++j) {
+      const intx8 k = {static_cast<int>(r.c[j][0]), static_cast<int>(r.c[j][1]),
+                       static_cast<int>(r.c[j][2]), static_cast<int>(r.c[j][3]), 0, 0, 0, 0};
+      const int scale = static_cast<int>(r.s[j]);  // 255: NaN
+      s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, q_lo[j], s, 4, 0, 0, scale, 1,
+                                                          q_scale[j]);
+      s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, q_hi[j], s, 4, 0, 0, scale, 0,
+                                                          q_scale[j]);
+    }
     return s;
   };
-  // Online softmax of the block's scores x (masked already): probabilities in x.
+  auto put_v = [&](const Raw& r) {
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      const float scale = __uint_as_float(r.s[i] << 23);
+      const uint32_t w[4] = {r.c[i][0], r.c[i][1], r.c[i][2], r.c[i][3]};
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        *reinterpret_cast<uint4*>(s_v + (v_at[i] ^ (16 * c))) = unpack8(w[c], scale);
+    }
+  };
+  // This thread's piece of a window into stage p of two.
+  const uint32_t w_at = w_row * ROWB + 16 * ((4 * v_blk) ^ swz_w<D>(w_row));
+  auto put_w = [&](const Raw& r, int p) {
+    if (!w_piece) return;
+    const float scale = __uint_as_float(r.s[0] << 23);  // 255: converts to NaN
+    const uint32_t w[4] = {r.c[0][0], r.c[0][1], r.c[0][2], r.c[0][3]};
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      *reinterpret_cast<uint4*>(sh.buf + p * kWindow * ROWB + (w_at ^ (16 * c))) =
+          unpack8(w[c], scale);
+  };
+  // Online softmax of the tile's scores x (masked already): probabilities in x.
   // The reference point st.m moves only when a lane's maximum grew by more than
   // kLazyLog2 in exp2 units (at most 2^kLazyLog2 is exact in bf16 and fp32).
-  auto softmax = [&](float (&x)[16]) {
+  auto softmax = [&](floatx16& x) {
     float tmax = x[0];
 #pragma unroll
     for (int r = 1; r < 16; ++r) tmax = fmaxf(tmax, x[r]);
@@ -260,172 +393,183 @@ __device__ __forceinline__ void attn_unit_mx4(const SgTreeAttnMx4Args& args, con
     }
     st.l += half_sum(psum);
   };
-  // O^T += V^T P^T over the block at LDS byte `at` of the V stages.
-  auto pv = [&](const float (&x)[16], int at) {
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      bf16x8 pf;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) pf[e] = static_cast<__bf16>(x[8 * c + e]);
-      const unsigned char* vrows = s_v + at + 8 * c * ROWB;
-#pragma unroll
-      for (int db = 0; db < DB; ++db) {
-        const short4_t lo =
-            __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(vrows + v_off[db][0]));
-        const short4_t hi =
-            __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(vrows + v_off[db][1]));
-        const short8_t v8 = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-        st.acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, v8), pf,
-                                                             st.acc[db], 0, 0, 0);
-      }
-    }
+  // V^T of half c of the tile's keys (a product's 16), at v0.  A wave's LDS accesses
+  // run in order, so the reads see the rows that its other lanes wrote before them.
+  struct Values {
+    short8_t v[DB];
   };
-  // Both steps of block b of the window in stage `stage`; limit: keys of the
-  // block that exist, bits: which of this lane's 16 keys its row sees.
-  auto block = [&](const floatx16& s, int at, int limit, uint32_t bits) {
-    float x[16];
+  auto read_v = [&](const unsigned char* v0, int c) {
+    Values r;
 #pragma unroll
-    for (int r = 0; r < 16; ++r)
-      x[r] = (16 * half + r < limit && ((bits >> r) & 1u)) ? s[r] : -__builtin_inff();
+    for (int db = 0; db < DB; ++db) {
+      const unsigned char* at = v0 + 8 * c * ROWB + (v_read ^ (64 * db));
+      const short4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)at);
+      const short4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(at + 4 * ROWB));
+      r.v[db] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    return r;
+  };
+  // O^T += V^T P^T over half c.
+  auto pv = [&](const floatx16& x, const Values& r, int c) {
+    bf16x8 pf;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) pf[e] = static_cast<__bf16>(x[8 * c + e]);
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+      st.acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, r.v[db]), pf,
+                                                           st.acc[db], 0, 0, 0);
+  };
+  // Softmax of the tile's scores x and the product with its V.  The first half of V
+  // is read before the softmax, the second while the first is multiplied (read
+  // after it, every product waited for its reads).
+  auto weigh = [&](floatx16& x, const unsigned char* v0) {
+    __builtin_amdgcn_wave_barrier();
+    const Values first = read_v(v0, 0);
     softmax(x);
-    pv(x, at);
+    const Values second = read_v(v0, 1);
+    pv(x, first, 0);
+    pv(x, second, 1);
+    __builtin_amdgcn_wave_barrier();
+  };
+  // The tile's keys from `limit` on, and those whose bit is off (bit r: this lane's
+  // key r), get the score -inf.
+  auto mask = [&](floatx16& x, int limit, uint32_t bits) {
+    const int mine = limit - 16 * half;  // keys of this lane's 16
+    bits &= mine >= 16 ? 0xffffu : mine > 0 ? (1u << mine) - 1u : 0u;
+    asm volatile("" : "+v"(bits));
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x[r] = ((bits >> r) & 1u) ? x[r] : -__builtin_inff();
   };
 
-  // The request's own rows, 64 at a time, through stage 0.  Parents precede
-  // their children: no row of the unit sees a tree key behind its last row.
+  // The request's own rows.  Parents precede their children: no row of the unit
+  // sees a tree key behind its last row.
+  uint32_t odd_tiles = 0u;  // tree tiles of this wave with a V that is no number
   if (do_tree) {
+    __syncthreads();  // the ancestor table is built
     const int tree_keys = u.row_begin + u.row_count;
     const int64_t tree0 = g * a.tree_head_stride + static_cast<int64_t>(r0) * a.tree_row_stride;
-    for (int key0 = 0; key0 < tree_keys; key0 += kWindow) {
-      const int key = min(key0 + p_row, n - 1);
-      uint4 v[LOADS][4];
+    const uint16_t* kt = static_cast<const uint16_t*>(a.k_tree_dev) + tree0;
+    const uint16_t* vt = static_cast<const uint16_t*>(a.v_tree_dev) + tree0;
+    // Q in bf16, columns 16 kb + 8 half .. +7.
+    bf16x8 qf[KB];
 #pragma unroll
-      for (int i = 0; i < LOADS; ++i) {
-        const bool is_v = D == 128 ? i == 1 : v_wave;
-        const uint16_t* src = static_cast<const uint16_t*>(is_v ? a.v_tree_dev : a.k_tree_dev) +
-                              tree0 + static_cast<int64_t>(key) * a.tree_row_stride + 32 * p_blk;
+    for (int kb = 0; kb < KB; ++kb)
+      qf[kb] = as_bf16x8(
+          q_valid ? *reinterpret_cast<const uint4*>(q_row + 16 * kb + 8 * half) : zero4());
+    for (int t = active ? ks : kAncWords; kTileKeys * t < tree_keys; t += streams) {
+      const int key0 = kTileKeys * t;
+      const uint16_t* kr =
+          kt + static_cast<int64_t>(min(key0 + k_key, n - 1)) * a.tree_row_stride + 8 * half;
+      uint4 v[P][4];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) v[i][c] = *reinterpret_cast<const uint4*>(src + 8 * c);
+      for (int i = 0; i < P; ++i) {
+        const uint16_t* vr =
+            vt + static_cast<int64_t>(min(key0 + v_row + kVStep * i, n - 1)) * a.tree_row_stride +
+            32 * v_blk;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) v[i][c] = *reinterpret_cast<const uint4*>(vr + 8 * c);
       }
-      __syncthreads();  // the stage is free; s_anc is built
+      floatx16 s;
 #pragma unroll
-      for (int i = 0; i < LOADS; ++i) {
-        const bool is_v = D == 128 ? i == 1 : v_wave;
-        uint32_t any = 0u;
+      for (int e = 0; e < 16; ++e) s[e] = 0.0f;
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+            as_bf16x8(*reinterpret_cast<const uint4*>(kr + 16 * kb)), qf[kb], s, 0, 0, 0);
+      uint32_t any = 0u;
+#pragma unroll
+      for (int i = 0; i < P; ++i)
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          if (is_v) {
-            // A value that is no number would reach every row of the block
-            // through a product with 0: it is added by itself at the end.
-            uint32_t w[4] = {v[i][c].x, v[i][c].y, v[i][c].z, v[i][c].w};
+          // A value that is no number would reach every row of the tile through a
+          // product with 0: it is added by itself at the end.
+          uint32_t w[4] = {v[i][c].x, v[i][c].y, v[i][c].z, v[i][c].w};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const uint32_t odd = nonfinite_halves(w[e]);
-              any |= odd;
-              w[e] &= ~odd;
-            }
-            v[i][c] = make_uint4(w[0], w[1], w[2], w[3]);
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t odd = nonfinite_halves(w[e]);
+            any |= odd;
+            w[e] &= ~odd;
           }
-          *reinterpret_cast<uint4*>(piece_at(i, c)) = v[i][c];
+          *reinterpret_cast<uint4*>(s_v + (v_at[i] ^ (16 * c))) =
+              make_uint4(w[0], w[1], w[2], w[3]);
         }
-        if (any != 0u) s_odd[(key0 + p_row) >> 5] = 1u;
-      }
-      __syncthreads();
-      if (!active) continue;
-      for (int b = streams == 2 ? ks : 0; b < (streams == 2 ? ks + 1 : 2); ++b) {
-        const int first = key0 + 32 * b;
-        if (first >= tree_keys) break;
-        block(qk(b * TILEB), b * TILEB, n - first, s_anc[r_local][first >> 5] >> (16 * half));
-      }
+      if (__ballot(any != 0u) != 0) odd_tiles |= 1u << t;
+      mask(s, n - key0, sh.anc[r_local][t] >> (16 * half));
+      weigh(s, s_v);
     }
-    __syncthreads();  // stage 0 is free
+    if (kShared) __syncthreads();  // the stages are free
   }
 
-  // The prefix.  Window w is read from stage w & 1 while window w + 1 is
-  // unpacked into the other one and w + 2 and w + 3 are on their way.
-  auto whole_block = [&](const floatx16& s, int at) {
-    float x[16];
-#pragma unroll
-    for (int r = 0; r < 16; ++r) x[r] = s[r];
-    softmax(x);
-    pv(x, at);
+  // The prefix.  This wave's codes two tiles on are on their way; where it takes
+  // every tile, its K one tile on (two sets of K registers did not fit: they spilled).
+  auto products = [&](int t, auto parity) {  // of tile t, whose K is in rk[parity]
+    constexpr int p = decltype(parity)::value;
+    constexpr int kAhead = kBoth ? 1 : 2;
+    const floatx16 s = qk(rk[p]);
+    if (t + kAhead * streams < tiles) load_k(t + kAhead * streams, rk[p]);
+    return s;
   };
-  auto step = [&](int w, auto parity) {
-    constexpr int p = decltype(parity)::value;  // w & 1
-    __syncthreads();
-    if (w + 1 < windows) {
-      unpack(raw[1 - p], 1 - p);
-      if (w + 3 < windows) load(w + 3, raw[1 - p]);
-    }
-    if (w == full || !active) return;
-    constexpr int at = p * STAGEB;
-    if constexpr (kTwo) {
-      const int mine = at + ks * TILEB;
-      whole_block(qk(mine), mine);
-    } else {
-      const floatx16 s0 = qk(at);
-      const floatx16 s1 = qk(at + TILEB);
-      whole_block(s0, at);
-      whole_block(s1, at + TILEB);
-    }
+  auto attend = [&](floatx16 x, int t, const unsigned char* v0) {
+    const int left = prefix_keys - t * kTileKeys;
+    if (left < kTileKeys) mask(x, left, 0xffffu);
+    weigh(x, v0);
   };
-  if (windows > 0) {
-    unpack(raw[0], 0);
-    if (windows > 2) load(2, raw[0]);
-  }
-  for (int w = 0; w < windows; w += 2) {
-    step(w, std::integral_constant<int, 0>{});
-    if (w + 1 < windows) step(w + 1, std::integral_constant<int, 1>{});
-  }
-  if (windows > full && active) {  // the last window, of fewer keys
-    const int left = prefix_keys - full * kWindow;
-    for (int b = streams == 2 ? ks : 0; b < (streams == 2 ? ks + 1 : 2); ++b) {
-      const int at = (full & 1) * STAGEB + b * TILEB;
-      if (32 * b < left) block(qk(at), at, left - 32 * b, 0xffffu);
+  using Even = std::integral_constant<int, 0>;
+  using Odd = std::integral_constant<int, 1>;
+  if constexpr (!kShared) {
+    auto step = [&](int t, auto parity) {
+      constexpr int p = decltype(parity)::value;
+      put_v(rv[p]);
+      if (t + 2 * streams < tiles) load_v(t + 2 * streams, rv[p]);
+      attend(products(t, parity), t, s_v);
+    };
+    for (int t = ks; t < tiles; t += 2 * streams) {
+      step(t, Even{});
+      if (t + streams < tiles) step(t + streams, Odd{});
+    }
+  } else {
+    auto window = [&](int w, auto parity) {
+      constexpr int p = decltype(parity)::value;
+      __syncthreads();  // stage p is whole, the other one read
+      if (w + 1 < windows) {
+        put_w(rv[1 - p], 1 - p);
+        if (w + 3 < windows) load_v(w + 3, rv[1 - p]);
+      }
+      const unsigned char* v0 = sh.buf + p * kWindow * ROWB;
+      if constexpr (kBoth) {
+        if (!active) return;
+        attend(products(2 * w, Even{}), 2 * w, v0);
+        if (2 * w + 1 >= tiles) return;
+        attend(products(2 * w + 1, Even{}), 2 * w + 1, v0 + kTileKeys * ROWB);
+      } else {
+        const int t = 2 * w + ks;
+        if (t < tiles) attend(products(t, parity), t, v0 + ks * kTileKeys * ROWB);
+      }
+    };
+    if (windows > 0) {
+      put_w(rv[0], 0);
+      if (windows > 2) load_v(2, rv[0]);
+    }
+    for (int w = 0; w < windows; w += 2) {
+      window(w, Even{});
+      if (w + 1 < windows) window(w + 1, Odd{});
     }
   }
-  __syncthreads();
 
-  // Merge the key streams of each q-group through LDS (the ring is free now).
-  auto merge_slot = [&](int q) { return reinterpret_cast<float*>(s_ring + q * kSlotBytes); };
-  if (active && ks > 0) {
-    float* slot = merge_slot(qg);
-    slot[lane] = st.m;
-    slot[64 + lane] = st.l;
-#pragma unroll
-    for (int db = 0; db < DB; ++db)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) slot[(2 + 16 * db + r) * 64 + lane] = st.acc[db][r];
-  }
-  __syncthreads();
-  if (!active || ks > 0) return;
-  if (streams == 2) {
-    const float* slot = merge_slot(qg);
-    const float ms = slot[lane];
-    const float m_all = fmaxf(st.m, ms);
-    const float m_use = (m_all == -__builtin_inff()) ? 0.0f : m_all;
-    const float w0 =
-        (st.m == -__builtin_inff()) ? 0.0f : __builtin_amdgcn_exp2f((st.m - m_use) * c2);
-    const float w1 = (ms == -__builtin_inff()) ? 0.0f : __builtin_amdgcn_exp2f((ms - m_use) * c2);
-    st.l = st.l * w0 + w1 * slot[64 + lane];
-#pragma unroll
-    for (int db = 0; db < DB; ++db)
-#pragma unroll
-      for (int r = 0; r < 16; ++r)
-        st.acc[db][r] = st.acc[db][r] * w0 + w1 * slot[(2 + 16 * db + r) * 64 + lane];
-    st.m = m_all;
-  }
-
-  // st.acc[db][r] holds head dim 32*db + 8*(r/4) + 4*half + (r%4) of this lane's query.
-  if (do_tree) {
-    const uint16_t* vt = static_cast<const uint16_t*>(a.v_tree_dev) + g * a.tree_head_stride +
-                         static_cast<int64_t>(r0) * a.tree_row_stride + 4 * half;
+  // st.acc[db][r] holds column 32*db + 8*(r/4) + 4*half + (r%4) of this lane's query.
+  if (odd_tiles != 0u) {
+    const ArgsIn z = fresh(in);
+    const int64_t tree_row_stride = z->attn.tree_row_stride;
+    const uint16_t* vt = static_cast<const uint16_t*>(z->attn.v_tree_dev) +
+                         g * z->attn.tree_head_stride +
+                         static_cast<int64_t>(r0) * tree_row_stride + 4 * half;
     for (int t = 0; t < kAncWords; ++t) {
-      if (s_odd[t] == 0u) continue;
-      const uint32_t word = s_anc[r_local][t];
+      if (((odd_tiles >> t) & 1u) == 0u) continue;
+      const uint32_t word = sh.anc[r_local][t];
 #pragma unroll 1
-      for (int j = 0; j < 32 && 32 * t + j < n; ++j) {
-        const uint16_t* vr = vt + static_cast<int64_t>(32 * t + j) * a.tree_row_stride;
+      for (int j = 0; j < kTileKeys && kTileKeys * t + j < n; ++j) {
+        const uint16_t* vr = vt + static_cast<int64_t>(kTileKeys * t + j) * tree_row_stride;
         const bool sees = ((word >> j) & 1u) != 0u;
 #pragma unroll
         for (int db = 0; db < DB; ++db)
@@ -443,10 +587,42 @@ __device__ __forceinline__ void attn_unit_mx4(const SgTreeAttnMx4Args& args, con
       }
     }
   }
+  __syncthreads();
+
+  // Merge the key streams of each q-group through LDS (the V tiles are done with).
+  if (active && ks > 0) {
+    float* slot = reinterpret_cast<float*>(sh.buf + ((ks - 1) * nq + qg) * Shared<D>::kSlot);
+    slot[lane] = st.m;
+    slot[64 + lane] = st.l;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) slot[(2 + 16 * db + r) * 64 + lane] = st.acc[db][r];
+  }
+  __syncthreads();
+  if (!active || ks > 0) return;
+  for (int k = 1; k < streams; ++k) {
+    const float* slot =
+        reinterpret_cast<const float*>(sh.buf + ((k - 1) * nq + qg) * Shared<D>::kSlot);
+    const float ms = slot[lane];
+    const float m_all = fmaxf(st.m, ms);
+    const float m_use = (m_all == -__builtin_inff()) ? 0.0f : m_all;
+    const float w0 =
+        (st.m == -__builtin_inff()) ? 0.0f : __builtin_amdgcn_exp2f((st.m - m_use) * c2);
+    const float w1 = (ms == -__builtin_inff()) ? 0.0f : __builtin_amdgcn_exp2f((ms - m_use) * c2);
+    st.l = st.l * w0 + w1 * slot[64 + lane];
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        st.acc[db][r] = st.acc[db][r] * w0 + w1 * slot[(2 + 16 * db + r) * 64 + lane];
+    st.m = m_all;
+  }
+
   if (u.partial >= 0) {
     // Partial layout (floats): O as float4 chunks ((db*4 + q4)*2 + half)*128 + m,
     // then the running max (log2 units) and sum per query vector.
-    float* part = static_cast<float*>(a.workspace_dev) + partial_floats(D) * u.partial;
+    float* part = static_cast<float*>(fresh(in)->attn.workspace_dev) + partial_floats(D) * u.partial;
     float4* o = reinterpret_cast<float4*>(part);
 #pragma unroll
     for (int db = 0; db < DB; ++db)
@@ -465,7 +641,7 @@ __device__ __forceinline__ void attn_unit_mx4(const SgTreeAttnMx4Args& args, con
   // Output through a staging tile of this wave (32 query vectors, rows padded by
   // 16 bytes), behind the merge slots where there are any.
   unsigned char* stage =
-      s_ring + (streams == 2 ? 2 * kSlotBytes : 0) + qg * 32 * kPitch;
+      sh.buf + (streams - 1) * nq * Shared<D>::kSlot + qg * Shared<D>::kStage;
   const float inv = st.l > 0.0f ? 1.0f / st.l : st.l;  // NaN stays NaN
 #pragma unroll
   for (int db = 0; db < DB; ++db)
@@ -478,34 +654,36 @@ __device__ __forceinline__ void attn_unit_mx4(const SgTreeAttnMx4Args& args, con
           packed;
     }
   __builtin_amdgcn_wave_barrier();
-  uint16_t* const out_base = static_cast<uint16_t*>(a.out_dev) +
-                             (static_cast<int64_t>(r0) + u.row_begin) * a.out_row_stride +
-                             static_cast<int64_t>(u.kv_head * G) * a.out_head_stride;
+  const ArgsIn o = fresh(in);
+  const int64_t out_row = o->attn.out_row_stride, out_head = o->attn.out_head_stride;
+  uint16_t* const out_base = static_cast<uint16_t*>(o->attn.out_dev) +
+                             (static_cast<int64_t>(r0) + u.row_begin) * out_row +
+                             static_cast<int64_t>(u.kv_head * G) * out_head;
   auto dst_of = [&](int q, int within) {
     const int mq = qg * 32 + q;
     const int rq = mq / G;
     return rq < u.row_count
-               ? out_base + static_cast<int64_t>(rq) * a.out_row_stride +
-                     static_cast<int64_t>(mq - rq * G) * a.out_head_stride + within / 2
+               ? out_base + static_cast<int64_t>(rq) * out_row +
+                     static_cast<int64_t>(mq - rq * G) * out_head + within / 2
                : nullptr;
   };
-  if (((a.out_row_stride | a.out_head_stride) & 7) == 0 &&
-      (reinterpret_cast<uintptr_t>(a.out_dev) & 15) == 0) {
+  if (((out_row | out_head) & 7) == 0 &&
+      (reinterpret_cast<uintptr_t>(o->attn.out_dev) & 15) == 0) {
 #pragma unroll
-    for (int i = 0; i < 32 * kRowBytes / 1024; ++i) {
+    for (int i = 0; i < 32 * ROWB / 1024; ++i) {
       const int linear = i * 1024 + 16 * lane;
-      const int q = linear / kRowBytes;
-      const int within = linear - q * kRowBytes;
+      const int q = linear / ROWB;
+      const int within = linear - q * ROWB;
       const uint4 v = *reinterpret_cast<const uint4*>(stage + q * kPitch + within);
       uint16_t* dst = dst_of(q, within);
       if (dst != nullptr) *reinterpret_cast<uint4*>(dst) = v;
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 32 * kRowBytes / 512; ++i) {
+    for (int i = 0; i < 32 * ROWB / 512; ++i) {
       const int linear = i * 512 + 8 * lane;
-      const int q = linear / kRowBytes;
-      const int within = linear - q * kRowBytes;
+      const int q = linear / ROWB;
+      const int within = linear - q * ROWB;
       const uint2 v = *reinterpret_cast<const uint2*>(stage + q * kPitch + within);
       uint16_t* dst = dst_of(q, within);
       if (dst != nullptr) *reinterpret_cast<uint2*>(dst) = v;
@@ -518,6 +696,7 @@ template <int D>
 __global__ __launch_bounds__(kThreads, 2) void tree_attn_mx4_kernel(SgTreeAttnMx4Args a,
                                                                      const AttnUnit* direct) {
   __shared__ Shared<D> sh;
+  const ArgsIn in = (ArgsIn)__builtin_amdgcn_kernarg_segment_ptr();
   const int group = a.attn.num_q_heads / a.attn.num_kv_heads;
   const AttnUnit* units = direct;
   int k = blockIdx.x;
@@ -532,10 +711,13 @@ __global__ __launch_bounds__(kThreads, 2) void tree_attn_mx4_kernel(SgTreeAttnMx
   }
   for (; k < end; ++k) {
     const AttnUnit u = units[k];
-    if (u.row_count * group <= 64) {
-      attn_unit_mx4<D, true>(a, u, sh);
+    const int vectors = u.row_count * group;
+    if (vectors <= 32) {
+      attn_unit_mx4<D, false, false>(a, in, u, sh);
+    } else if (vectors <= 64) {
+      attn_unit_mx4<D, true, false>(a, in, u, sh);
     } else {
-      attn_unit_mx4<D, false>(a, u, sh);
+      attn_unit_mx4<D, true, true>(a, in, u, sh);
     }
     __syncthreads();  // LDS of this unit is free before the next one starts
   }
