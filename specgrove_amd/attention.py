@@ -41,8 +41,9 @@ IMPLEMENTATION = "specgrove_hip"
 class PackedTreeMask:
     """Compact replacement of the packed dense mask."""
     pool: object                    # the prefixes: a PersistentRequestCachePool (arena per
-                                    # layer) or a PackedPrefix (non-persistent wave); both
-                                    # expose key_storage[l] / value_storage[l] [Hkv, T, D]
+                                    # layer) or a PackedPrefix (non-persistent wave), which
+                                    # expose key_storage[l] / value_storage[l] [Hkv, T, D],
+                                    # or a Mx4RequestCachePool (codes and scales)
     row_offset: torch.Tensor        # [n+1] i32, device
     parent: torch.Tensor            # [R] i32, request-local parents, -1 for roots
     prefix_start: torch.Tensor      # [n] i64, slot * capacity
@@ -183,6 +184,21 @@ def pack_block_inputs(states, blocks, cache_lengths: Sequence[int],
             {"full_attention": mask}, tuple(query_offsets))
 
 
+def attend(mask: PackedTreeMask, layer: int, q: torch.Tensor, k_tree: torch.Tensor,
+           v_tree: torch.Tensor, plan: ops.AttnPlan, *, out: torch.Tensor,
+           scale: float) -> torch.Tensor:
+    """Tree attention of one layer over the mask's prefixes as they are held: in 4
+    bits (a Mx4RequestCachePool) or in bf16."""
+    pool = mask.pool
+    meta = (mask.row_offset, mask.prefix_start, mask.prefix_len, mask.parent, plan)
+    if hasattr(pool, "k_codes"):
+        return ops.tree_attention_mx4(q, pool.k_codes[layer], pool.k_scales[layer],
+                                      pool.v_codes[layer], pool.v_scales[layer], k_tree,
+                                      v_tree, *meta, out=out, scale=scale)
+    return ops.tree_attention(q, pool.key_storage[layer], pool.value_storage[layer], k_tree,
+                              v_tree, *meta, out=out, scale=scale)
+
+
 def tree_attention_forward(module, query: torch.Tensor, key: torch.Tensor,
                            value: torch.Tensor, attention_mask, scaling: float | None = None,
                            dropout: float = 0.0, **kwargs):
@@ -206,15 +222,11 @@ def tree_attention_forward(module, query: torch.Tensor, key: torch.Tensor,
     hkv = key.shape[1]
     if rows != mask.num_rows or key.shape[2] != rows:
         raise ValueError("Packed rows disagree with the tree mask")
-    layer = module.layer_idx
-    k_cache = mask.pool.key_storage[layer]
-    v_cache = mask.pool.value_storage[layer]
     plan = mask.plan(hq, hkv, dim)
     out = torch.empty((1, rows, hq, dim), dtype=query.dtype, device=query.device)
-    ops.tree_attention(query[0].transpose(0, 1), k_cache, v_cache, key[0].transpose(0, 1),
-                       value[0].transpose(0, 1), mask.row_offset, mask.prefix_start,
-                       mask.prefix_len, mask.parent, plan, out=out[0],
-                       scale=scaling if scaling is not None else dim ** -0.5)
+    attend(mask, module.layer_idx, query[0].transpose(0, 1), key[0].transpose(0, 1),
+           value[0].transpose(0, 1), plan, out=out[0],
+           scale=scaling if scaling is not None else dim ** -0.5)
     return out, None
 
 

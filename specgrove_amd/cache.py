@@ -86,13 +86,11 @@ class PersistentRequestCacheLayer:
 
     @property
     def keys(self) -> torch.Tensor:
-        start, end = self._span()
-        return self._cache.pool.key_storage[self._layer_index][:, start:end].unsqueeze(0)
+        return self._cache.pool._cached_rows(self._layer_index, *self._span())[0].unsqueeze(0)
 
     @property
     def values(self) -> torch.Tensor:
-        start, end = self._span()
-        return self._cache.pool.value_storage[self._layer_index][:, start:end].unsqueeze(0)
+        return self._cache.pool._cached_rows(self._layer_index, *self._span())[1].unsqueeze(0)
 
 
 class PersistentRequestCache:
@@ -103,7 +101,7 @@ class PersistentRequestCache:
         self.pool = pool
         self.slot = slot
         self.layers = [PersistentRequestCacheLayer(self, i)
-                       for i in range(len(pool.key_storage))]
+                       for i in range(pool.num_layers)]
 
     def get_seq_length(self, layer_idx: int = 0) -> int:
         return self.pool.lengths[self.slot]
@@ -135,12 +133,24 @@ class PersistentRequestCachePool:
         first = caches[0].layers
         if any(layer.keys.shape[0] != 1 for cache in caches for layer in cache.layers):
             raise ValueError("Expected one request per source cache")
-        hkv, dim = first[0].keys.shape[1], first[0].keys.shape[-1]
         self.capacity = int(capacity)
         self.lengths = list(lengths)
-        arena = torch.empty((2, layers, hkv, len(caches) * self.capacity, dim),
-                            dtype=first[0].keys.dtype, device=first[0].keys.device)
-        for slot, (cache, length) in enumerate(zip(caches, lengths)):
+        self.num_layers = layers
+        self.device = first[0].keys.device
+        self._k_ptrs = None
+        self._v_ptrs = None
+        self._commit = None          # prepared commit call and its metadata buffers
+        self._status = None          # DeviceStatus of the commits, made by the first one
+        self._fill(caches)
+        self.caches = tuple(PersistentRequestCache(self, slot) for slot in range(len(caches)))
+
+    def _fill(self, caches: Sequence) -> None:
+        """Allocate the arena and copy the requests' prefills in."""
+        first = caches[0].layers[0].keys
+        hkv, dim = first.shape[1], first.shape[-1]
+        arena = torch.empty((2, self.num_layers, hkv, len(caches) * self.capacity, dim),
+                            dtype=first.dtype, device=first.device)
+        for slot, (cache, length) in enumerate(zip(caches, self.lengths)):
             if length == 0:
                 continue
             at = slice(slot * self.capacity, slot * self.capacity + length)
@@ -149,12 +159,10 @@ class PersistentRequestCachePool:
         self._arena = arena
         self.key_storage: list[torch.Tensor] = list(arena[0].unbind(0))
         self.value_storage: list[torch.Tensor] = list(arena[1].unbind(0))
-        self.device = arena.device
-        self.caches = tuple(PersistentRequestCache(self, slot) for slot in range(len(caches)))
-        self._k_ptrs = None
-        self._v_ptrs = None
-        self._commit = None          # prepared commit call and its metadata buffers
-        self._status = None          # DeviceStatus of the commits, made by the first one
+
+    def _cached_rows(self, layer: int, start: int, end: int):
+        """K and V [Hkv, end - start, D] of the arena's rows."""
+        return self.key_storage[layer][:, start:end], self.value_storage[layer][:, start:end]
 
     @property
     def status(self) -> DeviceStatus:
@@ -193,13 +201,8 @@ class PersistentRequestCachePool:
         host = torch.zeros(total, dtype=torch.int64, pin_memory=True)
         d32 = dev[2 * layers + cap:].view(torch.int32)
         base = cap + 1 + cap * stride
-        k_ptrs, v_ptrs = self._device_pointers()
-        k0 = self.key_storage[0]
-        call = ops.prepare_kv_commit(
-            k_ptrs[:layers], v_ptrs[:layers], dev[:layers], dev[layers:2 * layers],
-            num_kv_heads=k0.shape[0], head_dim=k0.shape[2],
-            cache_head_stride=k0.stride(0), cache_token_stride=k0.stride(1),
-            tree_row_stride=k0.shape[2], tree_head_stride=k0.shape[2],
+        call = self._prepare_commit(
+            layers, dev[:layers], dev[layers:2 * layers],
             row_offset=d32[:cap + 1], keep_rows=d32[cap + 1:base].view(cap, stride),
             keep_len=d32[base:base + cap], prefix_start=dev[2 * layers:2 * layers + cap],
             lengths=d32[base + cap:base + 2 * cap], capacity=self.capacity,
@@ -209,6 +212,16 @@ class PersistentRequestCachePool:
         self._commit = dict(call=call, dev=dev, host=host, layers=layers, slots=cap,
                             stride=stride, copied=copied)
         return self._commit
+
+    def _prepare_commit(self, layers: int, k_tree_ptrs: torch.Tensor,
+                        v_tree_ptrs: torch.Tensor, **metadata) -> ops.PreparedCall:
+        k_ptrs, v_ptrs = self._device_pointers()
+        k0 = self.key_storage[0]
+        return ops.prepare_kv_commit(
+            k_ptrs[:layers], v_ptrs[:layers], k_tree_ptrs, v_tree_ptrs,
+            num_kv_heads=k0.shape[0], head_dim=k0.shape[2],
+            cache_head_stride=k0.stride(0), cache_token_stride=k0.stride(1),
+            tree_row_stride=k0.shape[2], tree_head_stride=k0.shape[2], **metadata)
 
     def check_status(self) -> None:
         """Raise if a commit kernel reported an error (waits for the last
@@ -240,7 +253,7 @@ class PersistentRequestCachePool:
             raise ValueError("Persistent cache append metadata disagree")
         if int(packed_old_length) != packed.prefix_total:
             raise ValueError("Persistent cache append metadata disagree")
-        if len(packed.layers) != len(self.key_storage):
+        if len(packed.layers) != self.num_layers:
             raise ValueError("Persistent cache append metadata disagree")
         rows_total = packed.num_rows
         n = len(caches)
@@ -290,6 +303,106 @@ class PersistentRequestCachePool:
         self.status.after_launch()
         for slot, increment in increments:
             self.lengths[slot] += increment
+
+
+class Mx4RequestCachePool(PersistentRequestCachePool):
+    """A persistent arena in 4 bits: e2m1 codes with a power-of-two scale for each
+    32 values of a row (0.27 of the bf16 bytes), so that more or longer requests fit
+    and the attention reads less.
+
+    The interface is ``PersistentRequestCachePool``'s; it takes bf16 caches of
+    head_dim 64 or 128 on the GPU.  Prefills and kept rows are packed by
+    ``ops.kv_commit_mx4``, the attention is ``ops.tree_attention_mx4`` over
+    ``k_codes[l]`` / ``v_codes[l]`` [Hkv, slots * capacity, D/2] and ``k_scales[l]`` /
+    ``v_scales[l]`` [.., D/32]; a request's ``layers[l].keys`` / ``.values`` are its
+    rows unpacked into a new bf16 tensor, what the attention multiplies.
+    """
+
+    def _fill(self, caches: Sequence) -> None:
+        first = caches[0].layers[0].keys
+        hkv, dim = first.shape[1], first.shape[-1]
+        if dim not in (64, 128):
+            raise ValueError("A 4-bit cache needs head_dim 64 or 128")
+        for cache, length in zip(caches, self.lengths):
+            for layer in cache.layers:
+                for t in (layer.keys, layer.values):
+                    if t.dtype != torch.bfloat16 or t.device != first.device:
+                        raise ValueError("A 4-bit cache takes bf16 caches of one device")
+                    if t.shape != (1, hkv, length, dim):
+                        raise ValueError("Expected keys and values [1, Hkv, L, D]")
+        if first.device.type != "cuda":
+            raise ValueError("A 4-bit cache lives on the GPU")
+        slots = len(caches)
+        codes = torch.empty((2, self.num_layers, hkv, slots * self.capacity, dim // 2),
+                            dtype=torch.uint8, device=first.device)
+        scales = torch.empty((2, self.num_layers, hkv, slots * self.capacity, dim // 32),
+                             dtype=torch.uint8, device=first.device)
+        self._arena = (codes, scales)
+        self.k_codes, self.v_codes = list(codes[0].unbind(0)), list(codes[1].unbind(0))
+        self.k_scales, self.v_scales = list(scales[0].unbind(0)), list(scales[1].unbind(0))
+        # One call for a request's layers; its metadata and that of all requests go
+        # to the device in one copy: slot starts and tree pointers (int64), then row
+        # offsets, lengths to keep and lengths so far.
+        filled = [slot for slot in range(slots) if self.lengths[slot] > 0]
+        if not filled:
+            return
+        sources = [self._tree_rows(caches[slot]) for slot in filled]
+        words = np.zeros((len(filled), 3 + 2 * self.num_layers), np.int64)
+        for row, slot, tensors in zip(words, filled, sources):
+            row[0] = slot * self.capacity
+            row[1:3].view(np.int32)[:] = [0, self.lengths[slot], self.lengths[slot], 0]
+            row[3:] = [t.data_ptr() for t in tensors]
+        meta = ops.upload(words.reshape(-1), first.device).view(len(filled), -1)
+        for row, tensors in zip(meta, sources):
+            counts = row[1:3].view(torch.int32)
+            k0 = tensors[0]
+            self._prepare_commit(
+                self.num_layers, row[3:3 + self.num_layers], row[3 + self.num_layers:],
+                row_offset=counts[:2], keep_rows=None, keep_len=counts[2:3],
+                prefix_start=row[:1], lengths=counts[3:4], capacity=self.capacity,
+                status=self.status.dev).set(tree_row_stride=k0.stride(0),
+                                            tree_head_stride=k0.stride(1))()
+        self.status.after_launch()
+
+    def _tree_rows(self, cache) -> list[torch.Tensor]:
+        """K of every layer, then V, as [L, Hkv, D] views of one layout."""
+        tensors = [layer.keys[0] for layer in cache.layers]
+        tensors += [layer.values[0] for layer in cache.layers]
+        s = tensors[0].stride()
+        if s[2] != 1 or (s[0] | s[1]) % 8 or any(
+                t.stride() != s or t.data_ptr() % 16 for t in tensors):
+            tensors = [t.clone(memory_format=torch.contiguous_format) for t in tensors]
+        return [t.transpose(0, 1) for t in tensors]
+
+    def _cached_rows(self, layer: int, start: int, end: int):
+        return tuple(ops.kv_load_mx4(c[layer][:, start:end], s[layer][:, start:end])
+                     for c, s in ((self.k_codes, self.k_scales), (self.v_codes, self.v_scales)))
+
+    def _device_pointers(self):
+        if self._k_ptrs is None:
+            self._k_ptrs = (ops.pointer_array(self.k_codes, self.device),
+                            ops.pointer_array(self.k_scales, self.device))
+            self._v_ptrs = (ops.pointer_array(self.v_codes, self.device),
+                            ops.pointer_array(self.v_scales, self.device))
+        return self._k_ptrs, self._v_ptrs
+
+    def _prepare_commit(self, layers: int, k_tree_ptrs: torch.Tensor,
+                        v_tree_ptrs: torch.Tensor, **metadata) -> ops.PreparedCall:
+        (k_codes, k_scales), (v_codes, v_scales) = self._device_pointers()
+        c, s = self.k_codes[0], self.k_scales[0]
+        return ops.prepare_kv_commit_mx4(
+            k_codes[:layers], k_scales[:layers], v_codes[:layers], v_scales[:layers],
+            k_tree_ptrs, v_tree_ptrs, num_kv_heads=c.shape[0], head_dim=2 * c.shape[2],
+            code_head_stride=c.stride(0), code_token_stride=c.stride(1),
+            scale_head_stride=s.stride(0), scale_token_stride=s.stride(1),
+            tree_row_stride=2 * c.shape[2], tree_head_stride=2 * c.shape[2], **metadata)
+
+    def append_packed_sequence(self, packed: "TreeVerifyCache", *args, **kw) -> None:
+        """``PersistentRequestCachePool.append_packed_sequence``, packing the rows."""
+        if any(t.dtype != torch.bfloat16 or t.data_ptr() % 16
+               for layer in packed.layers for t in (layer.keys, layer.values)):
+            raise ValueError("A 4-bit cache takes 16-byte aligned bf16 rows")
+        super().append_packed_sequence(packed, *args, **kw)
 
 
 class _TreeLayer:

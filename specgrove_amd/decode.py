@@ -176,6 +176,7 @@ class WaveLoop:
                  max_new_tokens: int, stop_ids: Sequence[int] = (), row_cap: int = 64,
                  row_budget: int | None = None, slot_capacity: int | None = None,
                  persistent: bool = True, capacity: int | None = None, cache_factory=None,
+                 cache_format: str = "bf16",
                  tree_budget: int | None = None,
                  low_occupancy_row_cap: int | None = None,
                  low_occupancy_threshold: int | None = None,
@@ -207,6 +208,7 @@ class WaveLoop:
             max_new_tokens < 1 or row_cap < 1
             or (row_budget is not None and row_budget < row_cap)
             or (persistent and capacity is None)
+            or cache_format not in ("bf16", "mx4") or (cache_format == "mx4" and not persistent)
             or (adaptive_cap and (
                 low_occupancy_row_cap is None or low_occupancy_threshold is None
                 or (mid_occupancy_row_cap is None) != (mid_occupancy_threshold is None)
@@ -264,6 +266,7 @@ class WaveLoop:
         self.max_new_tokens, self.stops = max_new_tokens, {int(t) for t in stop_ids}
         self.row_cap, self.row_budget, self.slot_capacity = row_cap, row_budget, slot_capacity
         self.persistent, self.capacity, self.cache_factory = persistent, capacity, cache_factory
+        self.cache_format = cache_format
         self.tree_budget = budget
         self.low_occupancy_row_cap, self.low_occupancy_threshold = (low_occupancy_row_cap,
                                                                     low_occupancy_threshold)
@@ -310,7 +313,9 @@ class WaveLoop:
                                                             s.generated[-1] in self.stops):
                 s.done = True
         if self.persistent:
-            self.pool = cache_mod.PersistentRequestCachePool(
+            pool_of = (cache_mod.Mx4RequestCachePool if self.cache_format == "mx4"
+                       else cache_mod.PersistentRequestCachePool)
+            self.pool = pool_of(
                 [s.target_cache for s in states], self.capacity)
             for s, c in zip(states, self.pool.caches):
                 s.target_cache = c
@@ -534,7 +539,8 @@ def generate_tree_waves(model, states: Sequence[DecodeRequest], propose, *,
     ``row_budget``, ``slot_capacity``; ``persistent`` moves the caches into
     one ``PersistentRequestCachePool`` of ``capacity`` tokens per request (the
     reference's ``persistent_request_target_cache``), otherwise every wave
-    packs prefixes and splits the caches again; ``tree_budget`` with
+    packs prefixes and splits the caches again; ``cache_format="mx4"`` holds that
+    pool in 4 bits (``cache.Mx4RequestCachePool``); ``tree_budget`` with
     ``proposal_tree_budget``, ``low_occupancy_tree_budget`` /
     ``low_occupancy_tree_threshold`` / ``low_occupancy_expansion_slots``
     size the trees by occupancy; ``low_occupancy_row_cap`` /

@@ -3,7 +3,9 @@ HIP kernels: a Qwen3 causal LM (embedding, decoder layers, final norm, LM head)
 whose attention is the request-isolated tree attention over the persistent
 arena (or a non-persistent wave's packed prefixes), whose elementwise stages
 are the fused kernels of ``csrc/layer_ops.hip`` and whose projections are
-library GEMMs (hipBLASLt through ``torch.matmul``).
+library GEMMs (hipBLASLt through ``torch.matmul``) or, held in e4m3
+(``projections="fp8"``), the kernels of ``csrc/fp8_matmul.hip`` fed by the fp8
+forms of those stages (``csrc/fp8_rows.hip``).
 
 It replaces the transformers decoder that the reference runs per wave
 (``Engine.target_hidden_forward``, engine.py:499-517; transformers' Qwen3
@@ -152,16 +154,37 @@ def gather_rows(sources: Sequence[torch.Tensor], index: torch.Tensor) -> torch.T
     return out
 
 
+Weight = torch.Tensor | ops.PackedFp8Weight   # a projection, in bf16 or in e4m3
+
+
+def _in_fp8(weight: Weight) -> bool:
+    return isinstance(weight, ops.PackedFp8Weight)
+
+
+def _normed(weight: Weight, x: torch.Tensor, norm: torch.Tensor, eps: float,
+            residual: torch.Tensor | None):
+    """The add+RMSNorm in front of projection ``weight``: its rows, and the sum."""
+    stage = add_rmsnorm_fp8 if _in_fp8(weight) else add_rmsnorm
+    return stage(x, norm, eps, residual, want_sum=True)
+
+
+def _project(x: torch.Tensor | ops.Fp8Rows, weight: Weight) -> torch.Tensor:
+    """x @ weight.T in bf16."""
+    if _in_fp8(weight):
+        return ops.fp8_matmul(x if isinstance(x, ops.Fp8Rows) else ops.quantize_fp8(x), weight)
+    return torch.matmul(x, weight.T)
+
+
 @dataclass
 class _Layer:
     ln1: torch.Tensor
-    wqkv: torch.Tensor   # [(Hq + 2 Hkv) D, H]
+    wqkv: Weight         # [(Hq + 2 Hkv) D, H]
     q_norm: torch.Tensor
     k_norm: torch.Tensor
-    wo: torch.Tensor     # [H, Hq D]
+    wo: Weight           # [H, Hq D]
     ln2: torch.Tensor
-    wgu: torch.Tensor    # [2 I, H]
-    wd: torch.Tensor     # [H, I]
+    wgu: Weight          # [2 I, H]
+    wd: Weight           # [H, I]
 
 
 class _Head:
@@ -202,7 +225,13 @@ class Qwen3TargetStack:
         self.model = _Decoder(self)
 
     @classmethod
-    def from_transformers(cls, model) -> "Qwen3TargetStack":
+    def from_transformers(cls, model, projections: str = "bf16") -> "Qwen3TargetStack":
+        """The stack of a ``Qwen3ForCausalLM``.  ``projections="fp8"`` holds the
+        decoder layers' projections in e4m3 with a scale for each 128 x 128 block and
+        multiplies them with e4m3 rows (``ops.fp8_matmul``); embedding, norms and LM
+        head stay bf16."""
+        if projections not in ("bf16", "fp8"):
+            raise ValueError("projections must be 'bf16' or 'fp8'")
         cfg = model.config
         if getattr(cfg, "model_type", "qwen3") != "qwen3":
             raise ValueError("Qwen3TargetStack takes a Qwen3 causal LM")
@@ -215,6 +244,12 @@ class Qwen3TargetStack:
         def w(t):
             return t.detach().to(dtype).contiguous()
 
+        def proj(*parts):
+            weight = w(torch.cat(parts, 0)) if len(parts) > 1 else w(parts[0])
+            if projections == "bf16":
+                return weight
+            return ops.pack_fp8_weight(*ops.quantize_fp8_weight(weight))
+
         layers = []
         for layer in base.layers:
             attn, mlp = layer.self_attn, layer.mlp
@@ -223,12 +258,11 @@ class Qwen3TargetStack:
                 raise ValueError("Projections with bias are not implemented")
             layers.append(_Layer(
                 ln1=w(layer.input_layernorm.weight),
-                wqkv=w(torch.cat([attn.q_proj.weight, attn.k_proj.weight,
-                                  attn.v_proj.weight], 0)),
+                wqkv=proj(attn.q_proj.weight, attn.k_proj.weight, attn.v_proj.weight),
                 q_norm=w(attn.q_norm.weight), k_norm=w(attn.k_norm.weight),
-                wo=w(attn.o_proj.weight), ln2=w(layer.post_attention_layernorm.weight),
-                wgu=w(torch.cat([mlp.gate_proj.weight, mlp.up_proj.weight], 0)),
-                wd=w(mlp.down_proj.weight)))
+                wo=proj(attn.o_proj.weight), ln2=w(layer.post_attention_layernorm.weight),
+                wgu=proj(mlp.gate_proj.weight, mlp.up_proj.weight),
+                wd=proj(mlp.down_proj.weight)))
         theta = getattr(cfg, "rope_theta", None)
         if theta is None:
             theta = (getattr(cfg, "rope_parameters", None) or {}).get("rope_theta", 10000.0)
@@ -264,23 +298,23 @@ class Qwen3TargetStack:
         residual = None
         carry = x   # what the next add+RMSNorm adds to the residual stream
         for index, layer in enumerate(self.layers):
-            h, residual = add_rmsnorm(carry, layer.ln1, self.eps, residual, want_sum=True)
+            h, residual = _normed(layer.wqkv, carry, layer.ln1, self.eps, residual)
             if states is not None and index > 0:
                 states.append(residual)
-            qkv = torch.matmul(h, layer.wqkv.T)
+            qkv = _project(h, layer.wqkv)
             if index == 0:  # made while the GPU runs what is launched so far
                 plan = mask.plan(hq, hkv, d)
             q, k, v = qk_norm_rope(qkv, hq, hkv, d, layer.q_norm, layer.k_norm, self.inv_freq,
                                    positions, self.eps)
             k_new, v_new = cache.update(k[None], v[None], index)
             attn = torch.empty((rows, hq, d), dtype=x.dtype, device=x.device)
-            ops.tree_attention(q, mask.pool.key_storage[index], mask.pool.value_storage[index],
-                               k_new[0].transpose(0, 1), v_new[0].transpose(0, 1),
-                               mask.row_offset, mask.prefix_start, mask.prefix_len, mask.parent,
-                               plan, out=attn, scale=d ** -0.5)
-            o = torch.matmul(attn.view(rows, hq * d), layer.wo.T)
-            h, residual = add_rmsnorm(o, layer.ln2, self.eps, residual, want_sum=True)
-            carry = torch.matmul(silu_mul(torch.matmul(h, layer.wgu.T)), layer.wd.T)
+            attention.attend(mask, index, q, k_new[0].transpose(0, 1),
+                             v_new[0].transpose(0, 1), plan, out=attn, scale=d ** -0.5)
+            o = _project(attn.view(rows, hq * d), layer.wo)
+            h, residual = _normed(layer.wgu, o, layer.ln2, self.eps, residual)
+            gate_up = _project(h, layer.wgu)
+            carry = _project(silu_mul_fp8(gate_up) if _in_fp8(layer.wd) else silu_mul(gate_up),
+                             layer.wd)
         final = add_rmsnorm(carry, self.norm, self.eps, residual)
         if states is not None:
             states.append(final)
