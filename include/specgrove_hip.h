@@ -505,10 +505,18 @@ int sg_kv_load_mx4(const void* codes_dev, int64_t code_outer_stride, int64_t cod
                    void* out_dev, int64_t out_outer_stride, int64_t out_token_stride,
                    sg_stream_t stream);
 
+/* sg_tree_attn_plan for sg_tree_attn_mx4_fwd: the same records, cut for what the units
+ * take over a 4-bit prefix.  Either entry takes the plans of both. */
+int sg_tree_attn_plan_mx4(int32_t num_requests, const int32_t* row_offset_host,
+                          const int32_t* prefix_len_host, int32_t num_q_heads,
+                          int32_t num_kv_heads, int32_t head_dim, void* plan_host,
+                          size_t plan_capacity_bytes, size_t* plan_bytes, int32_t* plan_units,
+                          int32_t* plan_merges, size_t* workspace_bytes);
+
 /* sg_tree_attn_fwd over a 4-bit prefix (the wave's own rows are bf16). */
 typedef struct SgTreeAttnMx4Args {
   SgTreeAttnArgs attn;        /* k/v_cache_dev: codes, 16-byte aligned; the cache strides are
-                                 in bytes, multiples of 16.  Plans are sg_tree_attn_plan's */
+                                 in bytes, multiples of 16 */
   const void* k_scale_dev;    /* scales [Hkv, tokens, D/32] */
   const void* v_scale_dev;
   int64_t scale_head_stride, scale_token_stride;  /* bytes */

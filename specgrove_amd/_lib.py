@@ -183,6 +183,7 @@ EXPORTED_SYMBOLS = (
     "sg_lm_head_packed_bytes", "sg_lm_head_fresh",
     "sg_add_rmsnorm", "sg_qk_norm_rope", "sg_silu_mul", "sg_gather_rows",
     "sg_kv_commit_mx4", "sg_kv_load_mx4", "sg_tree_attn_mx4_fwd",
+    "sg_tree_attn_plan_mx4",
     "sg_fp8_quantize_rows", "sg_add_rmsnorm_fp8", "sg_silu_mul_fp8",
     "sg_fp8_packed_bytes", "sg_fp8_pack_weight", "sg_fp8_matmul",
     "sg_fp8_matmul_workspace_bytes",
@@ -216,6 +217,12 @@ def load() -> ctypes.CDLL:
     lib.sg_tree_attn_plan.restype = c_i32
     lib.sg_tree_attn_plan.argtypes = [
         c_i32, ctypes.POINTER(c_i32), ctypes.POINTER(c_i32), c_i32, c_i32, c_i32, c_i32,
+        c_void_p, c_size, ctypes.POINTER(c_size), ctypes.POINTER(c_i32),
+        ctypes.POINTER(c_i32), ctypes.POINTER(c_size),
+    ]
+    lib.sg_tree_attn_plan_mx4.restype = c_i32
+    lib.sg_tree_attn_plan_mx4.argtypes = [
+        c_i32, ctypes.POINTER(c_i32), ctypes.POINTER(c_i32), c_i32, c_i32, c_i32,
         c_void_p, c_size, ctypes.POINTER(c_size), ctypes.POINTER(c_i32),
         ctypes.POINTER(c_i32), ctypes.POINTER(c_size),
     ]

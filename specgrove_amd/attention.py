@@ -62,8 +62,10 @@ class PackedTreeMask:
         lets the wave's tensors outlive the current stream's use of them."""
         key = (num_q_heads, num_kv_heads, head_dim)
         if key not in self.plans:
-            plan = ops.plan_attention(self.row_offset_host, self.prefix_len_host, num_q_heads,
-                                      num_kv_heads, head_dim)
+            make = (ops.plan_attention_mx4 if hasattr(self.pool, "k_codes")
+                    else ops.plan_attention)
+            plan = make(self.row_offset_host, self.prefix_len_host, num_q_heads, num_kv_heads,
+                        head_dim)
             plan.device = ops.upload(plan.host, self.row_offset.device)
             self.plans[key] = plan
         plan = self.plans[key]

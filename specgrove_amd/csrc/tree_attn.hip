@@ -47,7 +47,6 @@
 namespace sg {
 namespace {
 
-constexpr int kListsPerCU = 2;                  // resident workgroups per CU
 // Shape of a workgroup.  kSmall: launches at D = 128 of at most one workgroup
 // per CU, whose units all have at most two q-groups.  Such a workgroup has all
 // of its CU and waits mostly for its copies: eight waves issue them, three
@@ -67,7 +66,6 @@ struct Shape {
   static constexpr int kAhead = kSmall ? 3 : 1;   // windows from a copy to its use
   static constexpr int kStages = 2 * kAhead + 2;  // tiles in each ring
 };
-constexpr int kDefaultCUs = 256;
 constexpr int64_t kSplitAbovePercent = 150;  // planner: split units above 1.5x a slot's share
 constexpr int64_t kRowSplitAbovePercent = 150;  // planner: units split by rows instead
 
@@ -857,6 +855,219 @@ __global__ __launch_bounds__(kMergeThreads) void tree_attn_merge_kernel(
 }  // namespace
 }  // namespace sg
 
+namespace sg {
+
+int check_plan_wave(const PlanWave& w, const PlanOut& out) {
+  SG_REQUIRE(w.num_requests >= 0, "num_requests must be non-negative");
+  SG_REQUIRE(w.num_requests == 0 || (w.row_offset && w.prefix_len), "null host array");
+  SG_REQUIRE(w.num_kv_heads >= 1 && w.num_q_heads >= w.num_kv_heads &&
+                 w.num_q_heads % w.num_kv_heads == 0,
+             "num_q_heads must be a positive multiple of num_kv_heads");
+  const int G = w.num_q_heads / w.num_kv_heads;
+  SG_REQUIRE(G <= kMaxGroup && kQPerUnit % G == 0,
+             "query heads per kv head must be 1, 2, 4, 8 or 16");
+  SG_REQUIRE(w.head_dim == 64 || w.head_dim == 128, "head_dim must be 64 or 128");
+  SG_REQUIRE(out.bytes && out.units && out.merges && out.workspace_bytes, "null output pointer");
+  SG_REQUIRE(w.num_requests == 0 || w.row_offset[0] == 0, "row_offset[0] must be 0");
+  for (int i = 0; i < w.num_requests; ++i) {
+    const int rows = w.row_offset[i + 1] - w.row_offset[i];
+    SG_REQUIRE(rows >= 0 && rows <= kMaxTreeRows,
+               "every request must have between 0 and 256 packed rows");
+    SG_REQUIRE(w.prefix_len[i] >= 0, "prefix lengths must be non-negative");
+  }
+  return SG_OK;
+}
+
+int emit_plan(const PlanWave& w, const PlanOut& out) {
+  const int G = w.num_q_heads / w.num_kv_heads;
+  const int rows_per_tile = kQPerUnit / G;
+  std::vector<AttnUnit> units;
+  std::vector<MergeGroup> merges;
+  int32_t partials = 0;
+  for (int i = 0; i < w.num_requests; ++i) {
+    const int rows = w.row_offset[i + 1] - w.row_offset[i];
+    if (rows == 0) continue;
+    const int L = w.prefix_len[i];
+    // A large unit with more than two q-groups is split by rows into units of
+    // 64 query vectors (half a row tile), which read the same K/V on one XCD
+    // (L2 serves the second read) and need no merge; only a unit of at most
+    // 64 query vectors is split over its prefix.
+    const bool row_split = w.split_rows[i] != 0;
+    const int rpt = row_split ? rows_per_tile / 2 : rows_per_tile;
+    const int splits = w.splits[i];
+    const int tiles = (rows + rpt - 1) / rpt;
+    for (int g = 0; g < w.num_kv_heads; ++g) {
+      for (int tile = 0; tile < tiles; ++tile) {
+        const int group = splits > 1 ? static_cast<int>(merges.size()) : -1;
+        const int first = partials;
+        for (int s = 0; s < splits; ++s) {
+          AttnUnit u;
+          u.req = i;
+          u.kv_head = g;
+          u.row_begin = tile * rpt;
+          u.row_count = std::min(rpt, rows - u.row_begin);
+          u.key_begin = static_cast<int32_t>(static_cast<int64_t>(L) * s / splits / kTileKeys *
+                                             kTileKeys);
+          u.key_end = s + 1 == splits ? L
+                                      : static_cast<int32_t>(static_cast<int64_t>(L) * (s + 1) /
+                                                             splits / kTileKeys * kTileKeys);
+          u.partial = splits > 1 ? partials++ : -1;
+          u.flags = ((s + 1 == splits) ? 1 : 0) | (row_split ? 2 : 0);
+          u.group = group;
+          u.num_splits = splits;
+          u.first_partial = splits > 1 ? first : -1;
+          u.pad = 0;
+          units.push_back(u);
+        }
+        if (splits > 1) {
+          MergeGroup mg;
+          mg.req = i;
+          mg.kv_head = g;
+          mg.row_begin = tile * rpt;
+          mg.row_count = std::min(rpt, rows - mg.row_begin);
+          mg.first_partial = first;
+          mg.num_partials = splits;
+          mg.pad0 = mg.pad1 = 0;
+          merges.push_back(mg);
+        }
+      }
+    }
+  }
+  // The order of the lists and the packing onto a given number of them go by the
+  // units' costs.  Every row tile is charged all tree tiles of its request, though the
+  // kernel stops at the tile's last row.
+  std::vector<int64_t> cost(units.size());
+  for (size_t k = 0; k < units.size(); ++k) {
+    const int rows = w.row_offset[units[k].req + 1] - w.row_offset[units[k].req];
+    const int64_t tiles =
+        (units[k].key_end - units[k].key_begin + kTileKeys - 1) / kTileKeys +
+        ((units[k].flags & 1) ? (rows + kTileKeys - 1) / kTileKeys : 0);
+    cost[k] = w.unit_cost(units[k].row_count, tiles);
+  }
+  std::vector<size_t> order(units.size());
+  std::iota(order.begin(), order.end(), size_t{0});
+  std::stable_sort(order.begin(), order.end(),
+                   [&](size_t x, size_t y) { return cost[x] > cost[y]; });
+  // By default every unit is a work list of its own, in decreasing cost
+  // order.  The first two per CU start at once, the largest on each CU's
+  // first slot (which the CU's issue arbitration favours), and the hardware
+  // dispatcher starts every further unit on the first slot that frees: greedy
+  // list scheduling at the speed each slot actually achieves.  With a target
+  // hint the units are packed onto that many lists instead.
+  const int64_t bins = w.lists > 0
+                           ? std::min<int64_t>(w.lists, static_cast<int64_t>(units.size()))
+                           : static_cast<int64_t>(units.size());
+  constexpr int64_t kXcds = 8;
+  std::vector<int64_t> load(bins, 0);
+  std::vector<std::vector<size_t>> bin_units(bins);
+  // Units that read the same (request, kv head) K/V (the row tiles of a tree
+  // larger than one tile, and split pieces) go to lists of one XCD: the
+  // dispatcher places workgroup b on XCD b % 8, whose L2 then serves the
+  // re-reads.  (A placement heuristic only.)
+  const size_t apart =
+      w.pieces_apart && !w.splits.empty()
+          ? std::max(1, *std::max_element(w.splits.begin(), w.splits.end()))
+          : 1;
+  std::vector<int64_t> xcd_of(static_cast<size_t>(w.num_requests) * w.num_kv_heads * apart, -1);
+  // The least loaded list (the first of equals) of each XCD's lists, or of all
+  // where there are fewer lists than XCDs, is the top of a heap: scanning the
+  // lists for every unit took half of a plan's time.
+  const int64_t classes = bins >= kXcds ? kXcds : 1;
+  using Entry = std::pair<int64_t, int64_t>;  // (load, list)
+  std::vector<std::priority_queue<Entry, std::vector<Entry>, std::greater<Entry>>> least(classes);
+  for (int64_t b = 0; b < bins; ++b) least[b % classes].push({0, b});
+  for (size_t k : order) {
+    size_t key = static_cast<size_t>(units[k].req) * w.num_kv_heads + units[k].kv_head;
+    if (w.pieces_apart && units[k].partial >= 0)
+      key = key * apart + (units[k].partial - units[k].first_partial);
+    else
+      key *= apart;
+    int64_t cls = 0;
+    if (xcd_of[key] >= 0 && classes > 1) {
+      cls = xcd_of[key];
+    } else {
+      for (int64_t c = 1; c < classes; ++c)
+        if (least[c].top() < least[cls].top()) cls = c;
+      xcd_of[key] = least[cls].top().second % kXcds;
+    }
+    const int64_t b = least[cls].top().second;
+    least[cls].pop();
+    load[b] += cost[k];
+    least[cls].push({load[b], b});
+    bin_units[b].push_back(k);
+  }
+  // Local search: move a unit out of the most loaded list, or swap it with a
+  // smaller unit of the least loaded list, while that lowers the maximum.
+  for (int round = 0; bins > 1 && round < 4096; ++round) {
+    const int64_t hi = std::max_element(load.begin(), load.end()) - load.begin();
+    const int64_t lo = std::min_element(load.begin(), load.end()) - load.begin();
+    const int64_t gap = load[hi] - load[lo];
+    int64_t best = 0;
+    size_t bi = 0, bj = SIZE_MAX;
+    for (size_t x = 0; x < bin_units[hi].size(); ++x) {
+      const int64_t cx = cost[bin_units[hi][x]];
+      if (cx < gap && cx > best) best = cx, bi = x, bj = SIZE_MAX;  // move
+      for (size_t y = 0; y < bin_units[lo].size(); ++y) {
+        const int64_t d = cx - cost[bin_units[lo][y]];
+        if (d > 0 && d < gap && d > best) best = d, bi = x, bj = y;  // swap
+      }
+    }
+    if (best == 0) break;
+    const size_t ux = bin_units[hi][bi];
+    if (bj == SIZE_MAX) {
+      bin_units[hi].erase(bin_units[hi].begin() + bi);
+      bin_units[lo].push_back(ux);
+    } else {
+      std::swap(bin_units[hi][bi], bin_units[lo][bj]);
+    }
+    load[hi] -= best;
+    load[lo] += best;
+  }
+  // Lists left empty by the XCD placement are dropped.
+  bin_units.erase(std::remove_if(bin_units.begin(), bin_units.end(),
+                                 [](const std::vector<size_t>& b) { return b.empty(); }),
+                  bin_units.end());
+  const int64_t lists = static_cast<int64_t>(bin_units.size());
+
+  const size_t bytes = sizeof(PlanHeader) + sizeof(AttnUnit) * units.size() +
+                       sizeof(MergeGroup) * merges.size() + sizeof(int32_t) * (lists + 1);
+  *out.bytes = bytes;
+  *out.units = static_cast<int32_t>(lists);
+  *out.merges = static_cast<int32_t>(merges.size());
+  *out.workspace_bytes = sizeof(float) * partial_floats(w.head_dim) * static_cast<size_t>(partials);
+  if (out.host == nullptr) return SG_OK;  // size query
+  SG_REQUIRE(out.capacity >= bytes, "plan buffer too small");
+  PlanHeader hdr = {};
+  hdr.magic = kPlanMagic;
+  hdr.num_units = static_cast<int32_t>(units.size());
+  hdr.num_merges = static_cast<int32_t>(merges.size());
+  hdr.rows_per_tile = rows_per_tile;
+  hdr.head_dim = w.head_dim;
+  hdr.group = G;
+  hdr.num_partials = partials;
+  hdr.num_bins = static_cast<int32_t>(lists);
+  hdr.num_requests = w.num_requests;
+  hdr.num_rows = w.num_requests > 0 ? w.row_offset[w.num_requests] : 0;
+  hdr.num_kv_heads = w.num_kv_heads;
+  for (const AttnUnit& u : units) hdr.unit_rows = std::max(hdr.unit_rows, u.row_count);
+  hdr.meta_hash = meta_hash(w.num_requests, w.row_offset, w.prefix_len);
+  char* bytes_out = static_cast<char*>(out.host);
+  std::memcpy(bytes_out, &hdr, sizeof(hdr));
+  AttnUnit* uo = reinterpret_cast<AttnUnit*>(bytes_out + sizeof(hdr));
+  MergeGroup* mo = reinterpret_cast<MergeGroup*>(uo + units.size());
+  int32_t* bo = reinterpret_cast<int32_t*>(mo + merges.size());
+  size_t next = 0;
+  for (int64_t b = 0; b < lists; ++b) {
+    bo[b] = static_cast<int32_t>(next);
+    for (size_t k : bin_units[b]) uo[next++] = units[k];
+  }
+  bo[lists] = static_cast<int32_t>(next);
+  std::memcpy(mo, merges.data(), sizeof(MergeGroup) * merges.size());
+  return SG_OK;
+}
+
+}  // namespace sg
+
 extern "C" int sg_tree_attn_plan(int32_t num_requests, const int32_t* row_offset_host,
                                  const int32_t* prefix_len_host, int32_t num_q_heads,
                                  int32_t num_kv_heads, int32_t head_dim,
@@ -866,18 +1077,13 @@ extern "C" int sg_tree_attn_plan(int32_t num_requests, const int32_t* row_offset
                                  size_t* workspace_bytes) {
   using namespace sg;
   clear_error();
-  SG_REQUIRE(num_requests >= 0, "num_requests must be non-negative");
-  SG_REQUIRE(num_requests == 0 || (row_offset_host && prefix_len_host), "null host array");
-  SG_REQUIRE(num_kv_heads >= 1 && num_q_heads >= num_kv_heads &&
-                 num_q_heads % num_kv_heads == 0,
-             "num_q_heads must be a positive multiple of num_kv_heads");
+  PlanWave wave = {num_requests, row_offset_host, prefix_len_host, num_q_heads, num_kv_heads,
+                   head_dim};
+  const PlanOut out = {plan_host,  plan_capacity_bytes, plan_bytes,
+                       plan_units, plan_merges,         workspace_bytes};
+  if (const int rc = check_plan_wave(wave, out)) return rc;
   const int G = num_q_heads / num_kv_heads;
-  SG_REQUIRE(G <= kMaxGroup && kQPerUnit % G == 0,
-             "query heads per kv head must be 1, 2, 4, 8 or 16");
-  SG_REQUIRE(head_dim == 64 || head_dim == 128, "head_dim must be 64 or 128");
-  SG_REQUIRE(plan_bytes && plan_units && plan_merges && workspace_bytes, "null output pointer");
   const int rows_per_tile = kQPerUnit / G;
-  SG_REQUIRE(num_requests == 0 || row_offset_host[0] == 0, "row_offset[0] must be 0");
 
   // Units of one (request, kv head, row tile) are split over their prefix when
   // the wave has too few units to give every CU slot work, or when one would
@@ -886,14 +1092,14 @@ extern "C" int sg_tree_attn_plan(int32_t num_requests, const int32_t* row_offset
   int64_t base_units = 0;
   for (int i = 0; i < num_requests; ++i) {
     const int rows = row_offset_host[i + 1] - row_offset_host[i];
-    SG_REQUIRE(rows >= 0 && rows <= kMaxTreeRows,
-               "every request must have between 0 and 256 packed rows");
-    SG_REQUIRE(prefix_len_host[i] >= 0, "prefix lengths must be non-negative");
     const int tiles = (rows + rows_per_tile - 1) / rows_per_tile;
     base_units += static_cast<int64_t>(num_kv_heads) * tiles;
   }
   const int64_t target = target_units_hint > 0 ? target_units_hint : kDefaultCUs * kListsPerCU;
-  auto unit_cost = [&](int row_count, int64_t tiles) -> int64_t {
+  // Hundredths of a microsecond on MI355X at 32q/8kv, D=128: a fixed part (prologue
+  // latency, epilogue) plus a part per 32-key tile; a unit with at most two q-groups
+  // (64 query vectors) streams two tiles per window and costs less per tile.
+  auto unit_cost = [G](int row_count, int64_t tiles) -> int64_t {
     const int nq = (row_count * G + 31) / 32;
     return nq <= 2 ? 550 + 57 * tiles : 840 + 88 * tiles;
   };
@@ -964,188 +1170,19 @@ extern "C" int sg_tree_attn_plan(int32_t num_requests, const int32_t* row_offset
       split_rows[i] = req_cost[i] > row_bound && rows * G > kQPerUnit / 2;
     }
   }
-  std::vector<AttnUnit> units;
-  std::vector<MergeGroup> merges;
-  int32_t partials = 0;
+  // Pieces keep at least four full tiles of prefix.
+  wave.lists = target_units_hint > 0 ? target : 0;
+  wave.unit_cost = unit_cost;
+  wave.splits.resize(num_requests);
+  wave.split_rows.resize(num_requests);
   for (int i = 0; i < num_requests; ++i) {
-    const int rows = row_offset_host[i + 1] - row_offset_host[i];
-    if (rows == 0) continue;
-    const int L = prefix_len_host[i];
-    // A large unit with more than two q-groups is split by rows into units of
-    // 64 query vectors (half a row tile), which read the same K/V on one XCD
-    // (L2 serves the second read) and need no merge; only a unit of at most
-    // 64 query vectors is split over its prefix.
     const bool row_split = !small_wave && split_rows[i] != 0;
-    const int rpt = row_split ? rows_per_tile / 2 : rows_per_tile;
-    // Pieces keep at least four full tiles of prefix.
-    const int splits =
-        small_wave ? small_splits[i]
-                   : std::max(1, std::min(row_split ? 1 : balance_splits[i], L / (4 * kTileKeys)));
-    const int tiles = (rows + rpt - 1) / rpt;
-    for (int g = 0; g < num_kv_heads; ++g) {
-      for (int tile = 0; tile < tiles; ++tile) {
-        const int group = splits > 1 ? static_cast<int>(merges.size()) : -1;
-        const int first = partials;
-        for (int s = 0; s < splits; ++s) {
-          AttnUnit u;
-          u.req = i;
-          u.kv_head = g;
-          u.row_begin = tile * rpt;
-          u.row_count = std::min(rpt, rows - u.row_begin);
-          u.key_begin = static_cast<int32_t>(static_cast<int64_t>(L) * s / splits / kTileKeys *
-                                             kTileKeys);
-          u.key_end = s + 1 == splits ? L
-                                      : static_cast<int32_t>(static_cast<int64_t>(L) * (s + 1) /
-                                                             splits / kTileKeys * kTileKeys);
-          u.partial = splits > 1 ? partials++ : -1;
-          u.flags = ((s + 1 == splits) ? 1 : 0) | (row_split ? 2 : 0);
-          u.group = group;
-          u.num_splits = splits;
-          u.first_partial = splits > 1 ? first : -1;
-          u.pad = 0;
-          units.push_back(u);
-        }
-        if (splits > 1) {
-          MergeGroup mg;
-          mg.req = i;
-          mg.kv_head = g;
-          mg.row_begin = tile * rpt;
-          mg.row_count = std::min(rpt, rows - mg.row_begin);
-          mg.first_partial = first;
-          mg.num_partials = splits;
-          mg.pad0 = mg.pad1 = 0;
-          merges.push_back(mg);
-        }
-      }
-    }
+    wave.split_rows[i] = row_split;
+    wave.splits[i] = small_wave ? small_splits[i]
+                                : std::max(1, std::min(row_split ? 1 : balance_splits[i],
+                                                       prefix_len_host[i] / (4 * kTileKeys)));
   }
-  // Unit cost, the order of the lists and the packing of a hinted list count
-  // (hundredths of a microsecond on MI355X at 32q/8kv, D=128): a fixed part
-  // (prologue latency, epilogue) plus a part per 32-key tile; a unit with at
-  // most two q-groups (64 query vectors) streams two tiles per window and
-  // costs less per tile.  Every row tile is charged all tree tiles of its
-  // request, here and in the splits above, though the kernel stops at the
-  // tile's last row.
-  std::vector<int64_t> cost(units.size());
-  for (size_t k = 0; k < units.size(); ++k) {
-    const int rows = row_offset_host[units[k].req + 1] - row_offset_host[units[k].req];
-    const int64_t tiles =
-        (units[k].key_end - units[k].key_begin + kTileKeys - 1) / kTileKeys +
-        ((units[k].flags & 1) ? (rows + kTileKeys - 1) / kTileKeys : 0);
-    cost[k] = unit_cost(units[k].row_count, tiles);
-  }
-  std::vector<size_t> order(units.size());
-  std::iota(order.begin(), order.end(), size_t{0});
-  std::stable_sort(order.begin(), order.end(),
-                   [&](size_t x, size_t y) { return cost[x] > cost[y]; });
-  // By default every unit is a work list of its own, in decreasing cost
-  // order.  The first two per CU start at once, the largest on each CU's
-  // first slot (which the CU's issue arbitration favours), and the hardware
-  // dispatcher starts every further unit on the first slot that frees: greedy
-  // list scheduling at the speed each slot actually achieves.  With a target
-  // hint the units are packed onto that many lists instead.
-  const int64_t bins = target_units_hint > 0
-                           ? std::min<int64_t>(target, static_cast<int64_t>(units.size()))
-                           : static_cast<int64_t>(units.size());
-  constexpr int64_t kXcds = 8;
-  std::vector<int64_t> load(bins, 0);
-  std::vector<std::vector<size_t>> bin_units(bins);
-  // Units that read the same (request, kv head) K/V (the row tiles of a tree
-  // larger than one tile, and split pieces) go to lists of one XCD: the
-  // dispatcher places workgroup b on XCD b % 8, whose L2 then serves the
-  // re-reads.  (A placement heuristic only.)
-  std::vector<int64_t> xcd_of(static_cast<size_t>(num_requests) * num_kv_heads, -1);
-  // The least loaded list (the first of equals) of each XCD's lists, or of all
-  // where there are fewer lists than XCDs, is the top of a heap: scanning the
-  // lists for every unit took half of a plan's time.
-  const int64_t classes = bins >= kXcds ? kXcds : 1;
-  using Entry = std::pair<int64_t, int64_t>;  // (load, list)
-  std::vector<std::priority_queue<Entry, std::vector<Entry>, std::greater<Entry>>> least(classes);
-  for (int64_t b = 0; b < bins; ++b) least[b % classes].push({0, b});
-  for (size_t k : order) {
-    const size_t key = static_cast<size_t>(units[k].req) * num_kv_heads + units[k].kv_head;
-    int64_t cls = 0;
-    if (xcd_of[key] >= 0 && classes > 1) {
-      cls = xcd_of[key];
-    } else {
-      for (int64_t c = 1; c < classes; ++c)
-        if (least[c].top() < least[cls].top()) cls = c;
-      xcd_of[key] = least[cls].top().second % kXcds;
-    }
-    const int64_t b = least[cls].top().second;
-    least[cls].pop();
-    load[b] += cost[k];
-    least[cls].push({load[b], b});
-    bin_units[b].push_back(k);
-  }
-  // Local search: move a unit out of the most loaded list, or swap it with a
-  // smaller unit of the least loaded list, while that lowers the maximum.
-  for (int round = 0; bins > 1 && round < 4096; ++round) {
-    const int64_t hi = std::max_element(load.begin(), load.end()) - load.begin();
-    const int64_t lo = std::min_element(load.begin(), load.end()) - load.begin();
-    const int64_t gap = load[hi] - load[lo];
-    int64_t best = 0;
-    size_t bi = 0, bj = SIZE_MAX;
-    for (size_t x = 0; x < bin_units[hi].size(); ++x) {
-      const int64_t cx = cost[bin_units[hi][x]];
-      if (cx < gap && cx > best) best = cx, bi = x, bj = SIZE_MAX;  // move
-      for (size_t y = 0; y < bin_units[lo].size(); ++y) {
-        const int64_t d = cx - cost[bin_units[lo][y]];
-        if (d > 0 && d < gap && d > best) best = d, bi = x, bj = y;  // swap
-      }
-    }
-    if (best == 0) break;
-    const size_t ux = bin_units[hi][bi];
-    if (bj == SIZE_MAX) {
-      bin_units[hi].erase(bin_units[hi].begin() + bi);
-      bin_units[lo].push_back(ux);
-    } else {
-      std::swap(bin_units[hi][bi], bin_units[lo][bj]);
-    }
-    load[hi] -= best;
-    load[lo] += best;
-  }
-  // Lists left empty by the XCD placement are dropped.
-  bin_units.erase(std::remove_if(bin_units.begin(), bin_units.end(),
-                                 [](const std::vector<size_t>& b) { return b.empty(); }),
-                  bin_units.end());
-  const int64_t lists = static_cast<int64_t>(bin_units.size());
-
-  const size_t bytes = sizeof(PlanHeader) + sizeof(AttnUnit) * units.size() +
-                       sizeof(MergeGroup) * merges.size() + sizeof(int32_t) * (lists + 1);
-  *plan_bytes = bytes;
-  *plan_units = static_cast<int32_t>(lists);
-  *plan_merges = static_cast<int32_t>(merges.size());
-  *workspace_bytes = sizeof(float) * partial_floats(head_dim) * static_cast<size_t>(partials);
-  if (plan_host == nullptr) return SG_OK;  // size query
-  SG_REQUIRE(plan_capacity_bytes >= bytes, "plan buffer too small");
-  PlanHeader hdr = {};
-  hdr.magic = kPlanMagic;
-  hdr.num_units = static_cast<int32_t>(units.size());
-  hdr.num_merges = static_cast<int32_t>(merges.size());
-  hdr.rows_per_tile = rows_per_tile;
-  hdr.head_dim = head_dim;
-  hdr.group = G;
-  hdr.num_partials = partials;
-  hdr.num_bins = static_cast<int32_t>(lists);
-  hdr.num_requests = num_requests;
-  hdr.num_rows = num_requests > 0 ? row_offset_host[num_requests] : 0;
-  hdr.num_kv_heads = num_kv_heads;
-  for (const AttnUnit& u : units) hdr.unit_rows = std::max(hdr.unit_rows, u.row_count);
-  hdr.meta_hash = meta_hash(num_requests, row_offset_host, prefix_len_host);
-  char* out = static_cast<char*>(plan_host);
-  std::memcpy(out, &hdr, sizeof(hdr));
-  AttnUnit* uo = reinterpret_cast<AttnUnit*>(out + sizeof(hdr));
-  MergeGroup* mo = reinterpret_cast<MergeGroup*>(uo + units.size());
-  int32_t* bo = reinterpret_cast<int32_t*>(mo + merges.size());
-  size_t next = 0;
-  for (int64_t b = 0; b < lists; ++b) {
-    bo[b] = static_cast<int32_t>(next);
-    for (size_t k : bin_units[b]) uo[next++] = units[k];
-  }
-  bo[lists] = static_cast<int32_t>(next);
-  std::memcpy(mo, merges.data(), sizeof(MergeGroup) * merges.size());
-  return SG_OK;
+  return emit_plan(wave, out);
 }
 
 extern "C" int sg_tree_attn_plan_check(const void* plan_host, int32_t num_requests,

@@ -3,6 +3,9 @@
 // checks of a unit against the call's metadata.
 #pragma once
 
+#include <functional>
+#include <vector>
+
 #include "sg_common.h"
 
 namespace sg {
@@ -22,6 +25,9 @@ constexpr int32_t kPlanMagic = 0x53475041;  // "SGPA"
 constexpr int kMaxGroup = 16;               // query heads per kv head
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazyLog2 = 8.0f;  // softmax reference point moves after a 2^8 growth
+
+constexpr int kListsPerCU = 2;                  // resident workgroups per CU
+constexpr int kDefaultCUs = 256;
 
 struct PlanHeader {
   int32_t magic;
@@ -233,6 +239,33 @@ struct AttnCall {
   int unit_rows;                   // most rows of a unit, 0 when not known
 };
 int check_attn_call(const SgTreeAttnArgs& a, AttnCall* call);
+
+// A wave to be planned: into how many prefix pieces each request's units are cut, which
+// requests' large units are cut by rows, and what a unit costs (in any measure, from its
+// rows and 32-key tiles).  lists: 0, or the number of work lists to pack the units onto.
+// pieces_apart: pieces of one prefix need not share an XCD (they share no keys).
+struct PlanWave {
+  int32_t num_requests;
+  const int32_t* row_offset;
+  const int32_t* prefix_len;
+  int32_t num_q_heads, num_kv_heads, head_dim;
+  int64_t lists = 0;
+  std::vector<int> splits;
+  std::vector<char> split_rows;
+  std::function<int64_t(int, int64_t)> unit_cost;
+  bool pieces_apart = false;
+};
+struct PlanOut {
+  void* host;  // nullptr: a size query
+  size_t capacity;
+  size_t* bytes;
+  int32_t* units;
+  int32_t* merges;
+  size_t* workspace_bytes;
+};
+int check_plan_wave(const PlanWave& wave, const PlanOut& out);
+// The plan's records (units, merge groups, work lists) into out.
+int emit_plan(const PlanWave& wave, const PlanOut& out);
 
 // Combines the plan's split partials (after the attention kernel).
 int launch_attn_merge(const SgTreeAttnArgs& a, const MergeGroup* groups, hipStream_t stream);

@@ -31,7 +31,11 @@
 // K and V unpacked to bf16 by the workgroup, 406 / 444 / 702; by each wave for
 // itself, 249 / 470 / 873; the products of a tile issued before the softmax of the
 // one before it, 583 / 381 / 672 (spills at one row).
+#include <algorithm>
+#include <cmath>
+#include <map>
 #include <type_traits>
+#include <vector>
 
 #include "tree_attn_common.h"
 
@@ -725,6 +729,162 @@ __global__ __launch_bounds__(kThreads, 2) void tree_attn_mx4_kernel(SgTreeAttnMx
 
 }  // namespace
 }  // namespace sg
+
+namespace sg {
+namespace {
+
+// What a unit takes, in microseconds on MI355X: a fixed part (prologue latency, Q's
+// terms, the tree, the epilogue) and a part per 64 keys, by its q-groups, with a second
+// unit on the CU or alone on it.  Measured over prefixes of 1,024 to 16,384 keys.
+struct UnitCost {
+  double fixed[2];
+  double window[2][4];
+};
+constexpr UnitCost kCost64 = {{6.0, 4.0}, {{0.55, 1.04, 1.84, 1.85}, {0.41, 0.89, 1.50, 1.56}}};
+constexpr UnitCost kCost128 = {{10.0, 8.0}, {{0.95, 1.69, 2.26, 2.51}, {0.72, 1.26, 1.75, 1.90}}};
+
+// The units of a wave by size: `count` of `micros` each.
+struct Alike {
+  double micros;
+  int64_t count;
+};
+
+// When the last of the units ends, if they start in decreasing size on `slots` slots.
+double end_of(std::vector<Alike>& units, int64_t slots) {
+  std::sort(units.begin(), units.end(),
+            [](const Alike& a, const Alike& b) { return a.micros > b.micros; });
+  std::map<double, int64_t> free;  // time -> slots that become free then
+  free[0.0] = slots;
+  double end = 0.0;
+  for (Alike u : units)
+    while (u.count > 0) {
+      const auto first = free.begin();
+      const double done = first->first + u.micros;
+      const int64_t taken = std::min(first->second, u.count);
+      u.count -= taken;
+      if ((first->second -= taken) == 0) free.erase(first);
+      free[done] += taken;
+      end = std::max(end, done);
+    }
+  return end;
+}
+
+}  // namespace
+}  // namespace sg
+
+// A unit in 4 bits takes a third to two thirds of its bf16 time per key but as long for
+// what is fixed, and a long one holds the launch's end up as much: prefixes are cut so
+// that the estimated end of the last unit, and of the merge that pieces need, is earliest.
+// Against the bf16 plan, 32 q / 8 kv heads, d = 128: 32 requests of 8,192-32,768 tokens
+// and 1 to 64 rows 443 us (736); 7 of 16,307-32,614 and one row 51 (65); 7 of 524-1,048
+// and 1 to 64 rows 25 (29); 64 of 512-4,096 and 16 to 128 rows 94 (92).
+extern "C" int sg_tree_attn_plan_mx4(int32_t num_requests, const int32_t* row_offset_host,
+                                     const int32_t* prefix_len_host, int32_t num_q_heads,
+                                     int32_t num_kv_heads, int32_t head_dim, void* plan_host,
+                                     size_t plan_capacity_bytes, size_t* plan_bytes,
+                                     int32_t* plan_units, int32_t* plan_merges,
+                                     size_t* workspace_bytes) {
+  using namespace sg;
+  clear_error();
+  PlanWave wave = {num_requests, row_offset_host, prefix_len_host, num_q_heads, num_kv_heads,
+                   head_dim};
+  const PlanOut out = {plan_host,  plan_capacity_bytes, plan_bytes,
+                       plan_units, plan_merges,         workspace_bytes};
+  if (const int rc = check_plan_wave(wave, out)) return rc;
+  const int G = num_q_heads / num_kv_heads;
+  const int rpt = kQPerUnit / G;
+  const UnitCost& cost = head_dim == 64 ? kCost64 : kCost128;
+  // A unit of `rows` rows over `keys` keys, and over its request's tree if it is the
+  // last piece.
+  auto micros = [&](int rows, double keys, int tree_rows, bool alone) {
+    const int nq = std::max(1, (rows * G + 31) / 32);
+    return cost.fixed[alone] + cost.window[alone][nq - 1] * (keys + tree_rows) / 64.0;
+  };
+  auto rows_of = [&](int i) { return row_offset_host[i + 1] - row_offset_host[i]; };
+
+  double total = 0.0;
+  int64_t whole = 0;
+  for (int i = 0; i < num_requests; ++i)
+    for (int r = 0; r < rows_of(i); r += rpt) {
+      total += num_kv_heads * micros(std::min(rpt, rows_of(i) - r), prefix_len_host[i],
+                                     rows_of(i), false);
+      whole += num_kv_heads;
+    }
+  constexpr int64_t kSlots = kDefaultCUs * kListsPerCU;
+  const double mean = std::max(1.0, (total - whole * cost.fixed[0]) / kSlots);
+  wave.splits.assign(num_requests, 1);
+  wave.split_rows.assign(num_requests, 0);
+  double best_end = 0.0;
+  std::vector<int> splits(num_requests, 1), last_splits;
+  std::vector<char> halves(num_requests, 0), last_halves;
+  std::vector<Alike> units;
+  // Whole units; then those above `share` of a slot's mean load cut by rows, into units
+  // of 64 query vectors, which need no merge but pass the keys twice; then by keys, into
+  // pieces of at most that load and at least 256 keys.
+  struct Cut {
+    bool by_rows;
+    double share;
+  };
+  constexpr Cut kCuts[] = {{false, 0.0},  {true, 2.0},   {true, 1.4},  {true, 1.0},  {false, 2.0},
+                           {false, 1.6},  {false, 1.35}, {false, 1.15}, {false, 1.05}, {false, 0.8},
+                           {false, 0.6}, {false, 0.45}, {false, 0.3}};
+  for (const Cut& cut : kCuts) {
+    int64_t count = 0;
+    double partial_bytes = 0.0;
+    for (int i = 0; i < num_requests; ++i) {
+      const int rows = rows_of(i);
+      if (rows == 0) continue;
+      const double keys_us =
+          micros(std::min(rows, rpt), prefix_len_host[i], 0, false) - cost.fixed[0];
+      halves[i] = cut.by_rows && keys_us > cut.share * mean && rows * G > kQPerUnit / 2;
+      splits[i] = 1;
+      if (!cut.by_rows && cut.share > 0.0)
+        splits[i] = static_cast<int>(std::max(1.0, std::min(std::ceil(keys_us / (cut.share * mean)),
+                                                            std::floor(prefix_len_host[i] / 256.0))));
+      const int of = halves[i] ? rpt / 2 : rpt;
+      count += static_cast<int64_t>((rows + of - 1) / of) * splits[i] * num_kv_heads;
+      if (splits[i] > 1)
+        partial_bytes += 4.0 * (head_dim + 2) * rows * num_q_heads * splits[i];
+    }
+    if (count > 8 * kSlots && cut.share > 0.0) continue;
+    if (splits == last_splits && halves == last_halves) continue;
+    last_splits = splits;
+    last_halves = halves;
+    const bool alone = count <= kDefaultCUs;
+    units.clear();
+    double load = 0.0;
+    for (int i = 0; i < num_requests; ++i) {
+      const int of = halves[i] ? rpt / 2 : rpt;
+      for (int r = 0; r < rows_of(i); r += of) {
+        const int rows = std::min(of, rows_of(i) - r);
+        const double keys = static_cast<double>(prefix_len_host[i]) / splits[i];
+        units.push_back({micros(rows, keys, rows_of(i), alone), num_kv_heads});
+        if (splits[i] > 1)
+          units.push_back({micros(rows, keys, 0, alone),
+                           static_cast<int64_t>(num_kv_heads) * (splits[i] - 1)});
+      }
+    }
+    for (const Alike& u : units) load += u.micros * u.count;
+    // The units that start first, the largest, run at nearly the speed of one on the CU
+    // (older waves issue first), and so do the last: seven eighths of the end at the
+    // speed of two, but no less than the slots' mean load.
+    double end = end_of(units, alone ? kDefaultCUs : kSlots);
+    if (!alone) end = std::max(load / kSlots, 0.88 * end);
+    if (partial_bytes > 0.0) end += 12.0 + partial_bytes / 4.5e6;  // the merge
+    if (cut.share == 0.0 || end < best_end) {
+      best_end = end;
+      wave.splits = splits;
+      wave.split_rows = halves;
+    }
+    // Whole units that come this near to an even load leave a cut nothing to gain.
+    if (cut.share == 0.0 && end < 1.1 * total / kSlots) break;
+  }
+  wave.pieces_apart = true;
+  wave.unit_cost = [&](int rows, int64_t tiles) {
+    return static_cast<int64_t>(100.0 * micros(rows, 32.0 * tiles, 0, false));
+  };
+  return emit_plan(wave, out);
+}
 
 extern "C" int sg_tree_attn_mx4_fwd(const SgTreeAttnMx4Args* args, sg_stream_t stream) {
   using namespace sg;

@@ -9,7 +9,7 @@ raise ValueError before anything is launched; launch errors raise RuntimeError.
 from __future__ import annotations
 
 import ctypes
-from dataclasses import dataclass, replace
+from dataclasses import dataclass, field, replace
 
 import numpy as np
 import torch
@@ -138,6 +138,9 @@ class AttnPlan:
     head_dim: int
     device: torch.Tensor | None = None
     workspace: torch.Tensor | None = None
+    # What the plan was made from, and the wave's plan over a 4-bit cache (in_mx4).
+    wave: tuple | None = field(default=None, repr=False, compare=False)
+    mx4: "AttnPlan | None" = field(default=None, repr=False, compare=False)
 
     @property
     def header(self) -> np.ndarray:
@@ -166,7 +169,25 @@ class AttnPlan:
         current stream's memory: calls that can overlap, as on two streams,
         must not share one."""
         return replace(self, workspace=torch.empty(
-            max(self.workspace_bytes, 16), dtype=torch.uint8, device=self.device.device))
+            max(self.workspace_bytes, 16), dtype=torch.uint8, device=self.device.device),
+            mx4=self.mx4.with_workspace() if self.mx4 is not None else None)
+
+    def in_mx4(self) -> "AttnPlan":
+        """The plan that ``tree_attention_mx4`` runs of this one: itself if it was made
+        for a 4-bit cache or a given number of units, else ``plan_attention_mx4`` of the
+        same wave, made and copied at the first use and kept (not while a stream is
+        captured: use the plan once before)."""
+        if self.wave is None:
+            return self
+        if self.mx4 is None:
+            _require(not torch.cuda.is_current_stream_capturing(),
+                     "the plan's 4-bit form is made at its first use: call once before a "
+                     "capture, or use plan_attention_mx4")
+            plan = plan_attention_mx4(*self.wave, self.num_q_heads, self.num_kv_heads,
+                                      self.head_dim)
+            plan.device = upload(plan.host, self.device.device)
+            self.mx4 = plan.with_workspace()
+        return self.mx4
 
 
 _PLAN_BYTES = 1 << 16  # about 1,300 units
@@ -174,7 +195,21 @@ _PLAN_BYTES = 1 << 16  # about 1,300 units
 
 def plan_attention(row_offset, prefix_len, num_q_heads: int, num_kv_heads: int,
                    head_dim: int, target_units: int = 0) -> AttnPlan:
-    lib = _lib.load()
+    return _make_plan("sg_tree_attn_plan", row_offset, prefix_len, num_q_heads, num_kv_heads,
+                      head_dim, target_units)
+
+
+def plan_attention_mx4(row_offset, prefix_len, num_q_heads: int, num_kv_heads: int,
+                       head_dim: int) -> AttnPlan:
+    """``plan_attention`` for ``tree_attention_mx4``: prefixes cut for what the units
+    take over a 4-bit cache."""
+    return _make_plan("sg_tree_attn_plan_mx4", row_offset, prefix_len, num_q_heads,
+                      num_kv_heads, head_dim)
+
+
+def _make_plan(entry: str, row_offset, prefix_len, num_q_heads: int, num_kv_heads: int,
+               head_dim: int, *hint: int) -> AttnPlan:
+    make = getattr(_lib.load(), entry)
     ro = np.ascontiguousarray(np.asarray(row_offset, dtype=np.int32))
     pl = np.ascontiguousarray(np.asarray(prefix_len, dtype=np.int32))
     n = int(pl.size)
@@ -185,21 +220,24 @@ def plan_attention(row_offset, prefix_len, num_q_heads: int, num_kv_heads: int,
     merges = ctypes.c_int32()
     ws = ctypes.c_size_t()
     args = (n, ro.ctypes.data_as(i32p), pl.ctypes.data_as(i32p), num_q_heads,
-            num_kv_heads, head_dim, target_units)
+            num_kv_heads, head_dim, *hint)
     # The plan is made once, into a buffer that holds most plans; the size it
     # reports serves a larger one.
     host = np.empty(_PLAN_BYTES, dtype=np.uint8)
     for _ in range(2):
-        rc = lib.sg_tree_attn_plan(*args, host.ctypes.data_as(ctypes.c_void_p), host.nbytes,
-                                   ctypes.byref(plan_bytes), ctypes.byref(units),
-                                   ctypes.byref(merges), ctypes.byref(ws))
+        rc = make(*args, host.ctypes.data_as(ctypes.c_void_p), host.nbytes,
+                  ctypes.byref(plan_bytes), ctypes.byref(units), ctypes.byref(merges),
+                  ctypes.byref(ws))
         if rc == 0 or plan_bytes.value <= host.nbytes:
             break
         host = np.empty(plan_bytes.value, dtype=np.uint8)
-    _lib.check(rc, "sg_tree_attn_plan")
+    _lib.check(rc, entry)
     host = host[:plan_bytes.value].copy()
-    return AttnPlan(host, units.value, merges.value, ws.value, num_q_heads,
+    plan = AttnPlan(host, units.value, merges.value, ws.value, num_q_heads,
                     num_kv_heads, head_dim)
+    if hint and hint[0] <= 0:  # cut by the planner's own rule: another cache, another cut
+        plan.wave = (ro.copy(), pl.copy())
+    return plan
 
 
 def check_plan(plan: AttnPlan, row_offset_host, prefix_len_host) -> None:
@@ -981,6 +1019,7 @@ def _mx4_attention_args(q, k_codes, k_scales, v_codes, v_scales, k_tree, v_tree,
                                row_offset, prefix_start, prefix_len, parent, plan, out, status)
     _require(fits, "the arguments do not fit together")
     check_plan_call(plan, n, rows, hq, hkv, dim)
+    plan = plan.in_mx4()
     if out is None:
         out = torch.empty((rows, hq, dim), dtype=bf16, device=q.device)
     os = out.stride()

@@ -172,3 +172,70 @@ def test_weights_quantized_on_the_host():
         for j in range(3):
             block = codes[128 * i:128 * i + 128, 128 * j:128 * j + 128].float()
             assert block.abs().max() in (0.0, 448.0)
+
+
+def _wave(seed):
+    import random
+    rng = random.Random(seed)
+    n = rng.choice([1, 2, 7, 40])
+    longest = rng.choice([40, 700, 9000, 40000])
+    lengths = [rng.choice([0, 1, rng.randint(0, longest), longest]) for _ in range(n)]
+    rows = [rng.choice([0, 1, 1, 16, 33, 64, 200, 256]) for _ in range(n)]
+    hq, hkv = rng.choice([(4, 2), (32, 8), (8, 8), (16, 1), (64, 8)])
+    return lengths, rows, hq, hkv, rng.choice([64, 128])
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_plans_over_a_4_bit_cache_cover_the_wave(seed):
+    """Every row tile of every request and kv head sees its whole prefix once, in pieces
+    of at least 256 keys, and its tree once; work lists and merge groups are whole."""
+    lengths, rows, hq, hkv, dim = _wave(seed)
+    offset = [0]
+    for r in rows:
+        offset.append(offset[-1] + r)
+    plan = ops.plan_attention_mx4(offset, lengths, hq, hkv, dim)
+    ops.check_plan(plan, offset, lengths)
+    header, units, merges, bins = ops.decode_plan(plan)
+    assert plan.units == len(bins) - 1 and plan.merges == len(merges)
+    if len(units):
+        assert bins[0] == 0 and bins[-1] == len(units) and (bins[1:] > bins[:-1]).all()
+    full = 128 // (hq // hkv)
+    # Rows of a unit: a full row tile, or half of one where the planner cut by rows.
+    tile = {int(u[0]): full // 2 if u[7] & 2 else full for u in units}
+    pieces, slots = {}, set()
+    for u in units.tolist():
+        req, head, row, count, begin, end, partial, flags, group, splits, first, _ = u
+        rpt = tile[req]
+        assert row % rpt == 0 and count == min(rpt, rows[req] - row)
+        assert flags & 2 == (2 if rpt < full else 0) and flags < 4
+        pieces.setdefault((req, head, row), []).append((begin, end, flags & 1, group, splits))
+        if partial >= 0:
+            assert partial not in slots and first <= partial < first + splits
+            slots.add(partial)
+            assert merges[group].tolist()[:6] == [req, head, row, count, first, splits]
+        else:
+            assert group == -1 and splits == 1
+    want = {(i, h, r) for i in range(len(rows)) for h in range(hkv)
+            for r in range(0, rows[i], tile.get(i, full))}
+    assert set(pieces) == want
+    for (req, _, _), p in pieces.items():
+        p.sort()
+        assert p[0][0] == 0 and p[-1][1] == lengths[req]
+        assert all(a[1] == b[0] for a, b in zip(p, p[1:]))
+        assert [x[2] for x in p] == [0] * (len(p) - 1) + [1]
+        assert all(x[4] == len(p) for x in p)
+        assert len(p) == 1 or all(x[1] - x[0] >= 224 for x in p)  # 256 less a 32-key tile
+    assert slots == set(range(len(slots)))
+    assert plan.workspace_bytes == 4 * 128 * (dim + 2) * len(slots)
+
+
+def test_a_long_unit_is_cut_for_4_bits_and_refusals():
+    plan = ops.plan_attention_mx4([0, 1, 2], [32768, 300], 32, 8, 128)
+    assert plan.merges > 0 and plan.in_mx4() is plan
+    given = ops.plan_attention([0, 1], [32768], 32, 8, 128, 5)
+    assert given.in_mx4() is given
+    for bad in (([0, 1], [-1], 32, 8, 128), ([0, 257], [5], 32, 8, 128), ([1, 2], [5], 32, 8, 128),
+                ([0, 1], [5], 32, 5, 128), ([0, 1], [5], 32, 8, 96), ([0, 1], [5, 6], 32, 8, 128)):
+        with pytest.raises(ValueError):
+            ops.plan_attention_mx4(*bad)
+    assert ops.plan_attention_mx4([0], [], 32, 8, 128).units == 0
