@@ -31,6 +31,14 @@ __device__ __forceinline__ Pair unpack(uint32_t v) {
   return {__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u)};
 }
 
+// a / (1 + exp(-a)), with the exponential of -|a| so that the divisor lies in [1, 2]:
+// the reciprocal instruction (1 ulp there) serves, where the division's ten
+// instructions took half of the kernel's issue time.
+__device__ __forceinline__ float silu(float a) {
+  const float e = expf(-fabsf(a));
+  return (a < 0.0f ? a * e : a) * __builtin_amdgcn_rcpf(1.0f + e);
+}
+
 struct RowsOut {
   unsigned char* codes;
   int64_t code_stride;
@@ -85,8 +93,8 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(const uint16_t* __re
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const Pair a = unpack(gv[k]), b = unpack(uv[k]);
-        v[2 * k] = a.lo / (1.0f + expf(-a.lo)) * b.lo;
-        v[2 * k + 1] = a.hi / (1.0f + expf(-a.hi)) * b.hi;
+        v[2 * k] = silu(a.lo) * b.lo;
+        v[2 * k + 1] = silu(a.hi) * b.hi;
       }
     } else {
 #pragma unroll
