@@ -200,7 +200,7 @@ __device__ __forceinline__ void attn_unit(const SgTreeAttnArgs& a, const AttnUni
   // tile and the planner did not split the rows (flags bit 1).
   const bool stream_kv = (u.flags & 2) == 0 && n * G <= kQPerUnit;
 
-  if (do_tree) build_ancestors(a, u, r0, n, s_run, s_anc);
+  if (do_tree) build_ancestors(u, load_parent(a, r0, n), s_run, s_anc);
 
   // Query operand: lane supplies Q[row, head, 16*kb + 8*half .. +7].
   bf16x8 qf[KB];

@@ -183,7 +183,14 @@ __device__ void poison_unit(const SgTreeAttnArgs& a, const AttnUnit& u, int r0) 
   }
 }
 
-// Ancestor-or-self bitsets of the tile's rows (request-local numbering).  A
+// One node per thread (n <= kMaxTreeRows <= threads): its parent.
+__device__ __forceinline__ int load_parent(const SgTreeAttnArgs& a, int r0, int n) {
+  const int tid = threadIdx.x;
+  return tid < n ? a.parent_dev[r0 + tid] : -1;
+}
+
+// Ancestor-or-self bitsets of the tile's rows (request-local numbering), from every
+// thread's load_parent().  A
 // row's walk to its root takes a run of consecutive nodes (parent = node - 1)
 // at a step: every step is a dependent LDS read and eight words of bits, and
 // a 256-row prompt chunk walked node by node spent ~17 us here, an eighth of
@@ -194,14 +201,11 @@ __device__ void poison_unit(const SgTreeAttnArgs& a, const AttnUnit& u, int r0) 
 // For workgroups of at least kMaxTreeRows threads; s_run [kMaxTreeRows] is
 // scratch (first node of each node's run, and that node's parent), s_anc
 // [kQPerUnit] is read after the caller's next barrier.
-__device__ __forceinline__ void build_ancestors(const SgTreeAttnArgs& a, const AttnUnit& u, int r0,
-                                                int n, int2* s_run,
+__device__ __forceinline__ void build_ancestors(const AttnUnit& u, int p, int2* s_run,
                                                 uint32_t (*s_anc)[kAncWords]) {
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   if (tid < kMaxTreeRows) {
-    // One node per thread (n <= kMaxTreeRows <= threads).
-    const int p = tid < n ? a.parent_dev[r0 + tid] : -1;
     const uint64_t linked = __ballot(lane > 0 && p == tid - 1);
     // The run starts at the highest unlinked lane at or below this one.
     const int start = 63 - __builtin_clzll(~linked & (~0ull >> (63 - lane)));

@@ -120,13 +120,14 @@ template <int D, bool kShared, bool kBoth>
 __device__ __forceinline__ void attn_unit_mx4(const SgTreeAttnMx4Args& args, ArgsIn in,
                                               const AttnUnit& u, Shared<D>& sh) {
   const SgTreeAttnArgs& a = args.attn;
-  constexpr int KB = D / 16;                  // QK^T products of 16 columns
   constexpr int DB = D / 32;                  // PV blocks of 32 columns
   constexpr int ROWB = D * 2;                 // bytes of an LDS row
   constexpr int P = D / 64;                   // 16-byte pieces of codes a lane loads of K (and V)
   constexpr int kPitch = ROWB + 16;
 
-  const int G = a.num_q_heads / a.num_kv_heads;
+  // Query heads of a kv head: 1, 2, 4, 8 or 16.
+  const int g_bits = __builtin_ctz(static_cast<unsigned>(a.num_q_heads / a.num_kv_heads));
+  const int G = 1 << g_bits;
   // Opaque, so that what follows from it is not kept in registers from one unit
   // of a list to the next.
   int tid = threadIdx.x;
@@ -151,13 +152,56 @@ __device__ __forceinline__ void attn_unit_mx4(const SgTreeAttnMx4Args& args, Arg
   const int ks = wave / nq;
   const bool active = ks < streams;
   const int m = qg * 32 + col;                // query vector inside the unit
-  const int r_local = m / G;
+  const int r_local = m >> g_bits;
   const int head = u.kv_head * G + (m - r_local * G);
   const bool q_valid = active && r_local < u.row_count;
   const int64_t row = static_cast<int64_t>(r0) + u.row_begin + r_local;
   const int g = u.kv_head;
   const bool do_tree = (u.flags & 1) != 0;
 
+  // What the start of the unit needs, loaded before the prefix's first codes: loads
+  // return in order, and one round trip serves all of it.
+  const int tree_keys = do_tree ? u.row_begin + u.row_count : 0;
+  const int parent = do_tree ? load_parent(a, r0, n) : -1;
+  // Q, bf16: piece [j][b][e] is columns 64 j + 32 b + 16 half + 8 e .. +7.
+  const uint16_t* const q_row = static_cast<const uint16_t*>(a.q_dev) + row * a.q_row_stride +
+                                static_cast<int64_t>(head) * a.q_head_stride;
+  auto q_piece = [&](int j, int b, int e) {
+    return q_valid ? *reinterpret_cast<const uint4*>(q_row + 64 * j + 32 * b + 16 * half + 8 * e)
+                   : zero4();
+  };
+  // Tree tile t: K of key pi(col) in the columns of q_raw, and V as it is written to LDS.
+  constexpr int kBlocks = D / 32;             // 32-column blocks of a row
+  const int v_row = lane / kBlocks;           // of piece 0; piece i: + 64 / kBlocks
+  const int v_blk = lane % kBlocks;
+  constexpr int kVStep = 64 / kBlocks;
+  const int k_key = key_pi(col);
+  struct TreeTile {
+    uint4 k[P][2][2], v[P][4];
+  };
+  auto load_tree = [&](int t, TreeTile& tile) {
+    const int64_t tree0 = g * a.tree_head_stride + static_cast<int64_t>(r0) * a.tree_row_stride;
+    const int key0 = kTileKeys * t;
+    const uint16_t* kr = static_cast<const uint16_t*>(a.k_tree_dev) + tree0 +
+                         static_cast<int64_t>(min(key0 + k_key, n - 1)) * a.tree_row_stride +
+                         16 * half;
+#pragma unroll
+    for (int j = 0; j < P; ++j)
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          tile.k[j][b][e] = *reinterpret_cast<const uint4*>(kr + 64 * j + 32 * b + 8 * e);
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      const uint16_t* vr =
+          static_cast<const uint16_t*>(a.v_tree_dev) + tree0 +
+          static_cast<int64_t>(min(key0 + v_row + kVStep * i, n - 1)) * a.tree_row_stride +
+          32 * v_blk;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tile.v[i][c] = *reinterpret_cast<const uint4*>(vr + 8 * c);
+    }
+  };
   // Codes and scales of this lane.  K: of key pi(col) of a tile, piece j holds
   // columns 64 j + 32 half .. +31, an operand of product j.  V: piece i is 32
   // columns of a row, of a tile or (shared) of a window's 64 keys.
@@ -177,11 +221,6 @@ __device__ __forceinline__ void attn_unit_mx4(const SgTreeAttnMx4Args& args, Arg
   uint32_t c_stride = static_cast<uint32_t>(a.cache_token_stride);
   uint32_t s_stride = static_cast<uint32_t>(args.scale_token_stride);
   asm volatile("" : "+s"(c_stride), "+s"(s_stride));
-  const int k_key = key_pi(col);
-  constexpr int kBlocks = D / 32;             // 32-column blocks of a row
-  const int v_row = lane / kBlocks;           // of piece 0; piece i: + 64 / kBlocks
-  const int v_blk = lane % kBlocks;
-  constexpr int kVStep = 64 / kBlocks;
   constexpr int kWindow = 2 * kTileKeys;      // keys of a shared stage
   const int w_row = tid / kBlocks;            // of a window's piece, below kWindow
   const bool w_piece = kWindow * kBlocks >= kThreads || wave < kWindow * kBlocks / 64;
@@ -247,61 +286,7 @@ __device__ __forceinline__ void attn_unit_mx4(const SgTreeAttnMx4Args& args, Arg
     if (ks + streams < tiles) load_v(ks + streams, rv[1]);
   }
 
-  if (do_tree) build_ancestors(a, u, r0, n, sh.run, sh.anc);
-
-  // The query vector in two 8-bit terms.  Product j takes columns 64 j .. +63: this
-  // lane's bytes 0-15 are columns 64 j + 16 half .. +15, bytes 16-31 those 32 on;
-  // the scale of block b (32 columns) is read from lane half b.
-  const uint16_t* const q_row = static_cast<const uint16_t*>(a.q_dev) + row * a.q_row_stride +
-                                static_cast<int64_t>(head) * a.q_head_stride;
-  intx8 q_hi[P], q_lo[P];
-  int q_scale[P];  // bytes 0, 1: of hi and lo
-#pragma unroll
-  for (int j = 0; j < P; ++j) {
-    int code[2];
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      uint32_t w[8];
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const uint4 v = q_valid ? *reinterpret_cast<const uint4*>(q_row + 64 * j + 32 * b +
-                                                                  16 * half + 8 * e)
-                                : zero4();
-        w[4 * e] = v.x, w[4 * e + 1] = v.y, w[4 * e + 2] = v.z, w[4 * e + 3] = v.w;
-      }
-      uint32_t most = 0u;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) most = max(max(most, (w[e] << 16) & 0x7fffffffu),
-                                             w[e] & 0x7fff0000u);
-      const auto both = __builtin_amdgcn_permlane32_swap(most, most, false, false);
-      const int top = static_cast<int>(max(both[0], both[1]) >> 23);
-      code[b] = min(max(top - 7, 5), 254);  // the largest magnitude is below 256
-      const float x_hi = __uint_as_float(static_cast<uint32_t>(code[b]) << 23);
-      const float x_lo = __uint_as_float(static_cast<uint32_t>(code[b] - 4) << 23);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        short2_t hi = {0, 0}, lo = {0, 0};
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const uint32_t whole = w[2 * e + k], head4 = whole & 0xfff0fff0u;
-          const float lo0 = __uint_as_float(whole << 16) - __uint_as_float(head4 << 16);
-          const float lo1 =
-              __uint_as_float(whole & 0xffff0000u) - __uint_as_float(head4 & 0xffff0000u);
-          if (k == 0) {
-            hi = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(hi, as_pair(head4), x_hi, false);
-            lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(lo, lo0, lo1, x_lo, false);
-          } else {
-            hi = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(hi, as_pair(head4), x_hi, true);
-            lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(lo, lo0, lo1, x_lo, true);
-          }
-        }
-        // An infinity or a NaN: the block is NaN.
-        q_hi[j][4 * b + e] = top == 255 ? 0x7f7f7f7f : __builtin_bit_cast(int, hi);
-        q_lo[j][4 * b + e] = __builtin_bit_cast(int, lo);
-      }
-    }
-    q_scale[j] = half == 0 ? code[0] | (code[0] - 4) << 8 : code[1] | (code[1] - 4) << 8;
-  }
+  if (do_tree) build_ancestors(u, parent, sh.run, sh.anc);
 
   // LDS of this wave's V tile.  Chunk c of row r is at c ^ swz(r): a block's chunk c
   // is at its first one's address ^ 16 c.
@@ -331,22 +316,6 @@ __device__ __forceinline__ void attn_unit_mx4(const SgTreeAttnMx4Args& args, Arg
 #pragma unroll
     for (int r = 0; r < 16; ++r) st.acc[db][r] = 0.0f;
 
-  auto qk = [&](const Raw& r) {
-    floatx16 s;
-#pragma unroll
-    for (int e = 0; e < 16; ++e) s[e] = 0.0f;
-#pragma unroll
-    for (int j = 0; j < P; ++j) {
-      const intx8 k = {static_cast<int>(r.c[j][0]), static_cast<int>(r.c[j][1]),
-                       static_cast<int>(r.c[j][2]), static_cast<int>(r.c[j][3]), 0, 0, 0, 0};
-      const int scale = static_cast<int>(r.s[j]);  // 255: NaN
-      s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, q_lo[j], s, 4, 0, 0, scale, 1,
-                                                          q_scale[j]);
-      s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, q_hi[j], s, 4, 0, 0, scale, 0,
-                                                          q_scale[j]);
-    }
-    return s;
-  };
   auto put_v = [&](const Raw& r) {
 #pragma unroll
     for (int i = 0; i < P; ++i) {
@@ -451,36 +420,28 @@ __device__ __forceinline__ void attn_unit_mx4(const SgTreeAttnMx4Args& args, Arg
   uint32_t odd_tiles = 0u;  // tree tiles of this wave with a V that is no number
   if (do_tree) {
     __syncthreads();  // the ancestor table is built
-    const int tree_keys = u.row_begin + u.row_count;
-    const int64_t tree0 = g * a.tree_head_stride + static_cast<int64_t>(r0) * a.tree_row_stride;
-    const uint16_t* kt = static_cast<const uint16_t*>(a.k_tree_dev) + tree0;
-    const uint16_t* vt = static_cast<const uint16_t*>(a.v_tree_dev) + tree0;
-    // Q in bf16, columns 16 kb + 8 half .. +7.
-    bf16x8 qf[KB];
+    uint4 q_raw[P][2][2];
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb)
-      qf[kb] = as_bf16x8(
-          q_valid ? *reinterpret_cast<const uint4*>(q_row + 16 * kb + 8 * half) : zero4());
+    for (int j = 0; j < P; ++j)
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) q_raw[j][b][e] = q_piece(j, b, e);
     for (int t = active ? ks : kAncWords; kTileKeys * t < tree_keys; t += streams) {
+      TreeTile tree;
+      load_tree(t, tree);
       const int key0 = kTileKeys * t;
-      const uint16_t* kr =
-          kt + static_cast<int64_t>(min(key0 + k_key, n - 1)) * a.tree_row_stride + 8 * half;
-      uint4 v[P][4];
-#pragma unroll
-      for (int i = 0; i < P; ++i) {
-        const uint16_t* vr =
-            vt + static_cast<int64_t>(min(key0 + v_row + kVStep * i, n - 1)) * a.tree_row_stride +
-            32 * v_blk;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) v[i][c] = *reinterpret_cast<const uint4*>(vr + 8 * c);
-      }
       floatx16 s;
 #pragma unroll
       for (int e = 0; e < 16; ++e) s[e] = 0.0f;
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
-        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-            as_bf16x8(*reinterpret_cast<const uint4*>(kr + 16 * kb)), qf[kb], s, 0, 0, 0);
+      for (int j = 0; j < P; ++j)
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                as_bf16x8(tree.k[j][b][e]), as_bf16x8(q_raw[j][b][e]), s, 0, 0, 0);
       uint32_t any = 0u;
 #pragma unroll
       for (int i = 0; i < P; ++i)
@@ -488,7 +449,7 @@ __device__ __forceinline__ void attn_unit_mx4(const SgTreeAttnMx4Args& args, Arg
         for (int c = 0; c < 4; ++c) {
           // A value that is no number would reach every row of the tile through a
           // product with 0: it is added by itself at the end.
-          uint32_t w[4] = {v[i][c].x, v[i][c].y, v[i][c].z, v[i][c].w};
+          uint32_t w[4] = {tree.v[i][c].x, tree.v[i][c].y, tree.v[i][c].z, tree.v[i][c].w};
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const uint32_t odd = nonfinite_halves(w[e]);
@@ -505,6 +466,72 @@ __device__ __forceinline__ void attn_unit_mx4(const SgTreeAttnMx4Args& args, Arg
     if (kShared) __syncthreads();  // the stages are free
   }
 
+  // The query vector in two 8-bit terms.  Product j takes columns 64 j .. +63: this
+  // lane's bytes 0-15 are columns 64 j + 16 half .. +15, bytes 16-31 those 32 on;
+  // the scale of block b (32 columns) is read from lane half b.
+  intx8 q_hi[P], q_lo[P];
+  int q_scale[P];  // bytes 0, 1: of hi and lo
+#pragma unroll
+  for (int j = 0; j < P; ++j) {
+    int code[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      uint32_t w[8];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const uint4 v = q_piece(j, b, e);
+        w[4 * e] = v.x, w[4 * e + 1] = v.y, w[4 * e + 2] = v.z, w[4 * e + 3] = v.w;
+      }
+      uint32_t most = 0u;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) most = max(max(most, (w[e] << 16) & 0x7fffffffu),
+                                             w[e] & 0x7fff0000u);
+      const auto both = __builtin_amdgcn_permlane32_swap(most, most, false, false);
+      const int top = static_cast<int>(max(both[0], both[1]) >> 23);
+      code[b] = min(max(top - 7, 5), 254);  // the largest magnitude is below 256
+      const float x_hi = __uint_as_float(static_cast<uint32_t>(code[b]) << 23);
+      const float x_lo = __uint_as_float(static_cast<uint32_t>(code[b] - 4) << 23);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        short2_t hi = {0, 0}, lo = {0, 0};
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const uint32_t whole = w[2 * e + k], head4 = whole & 0xfff0fff0u;
+          const float lo0 = __uint_as_float(whole << 16) - __uint_as_float(head4 << 16);
+          const float lo1 =
+              __uint_as_float(whole & 0xffff0000u) - __uint_as_float(head4 & 0xffff0000u);
+          if (k == 0) {
+            hi = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(hi, as_pair(head4), x_hi, false);
+            lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(lo, lo0, lo1, x_lo, false);
+          } else {
+            hi = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(hi, as_pair(head4), x_hi, true);
+            lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(lo, lo0, lo1, x_lo, true);
+          }
+        }
+        // An infinity or a NaN: the block is NaN.
+        q_hi[j][4 * b + e] = top == 255 ? 0x7f7f7f7f : __builtin_bit_cast(int, hi);
+        q_lo[j][4 * b + e] = __builtin_bit_cast(int, lo);
+      }
+    }
+    q_scale[j] = half == 0 ? code[0] | (code[0] - 4) << 8 : code[1] | (code[1] - 4) << 8;
+  }
+
+  auto qk = [&](const Raw& r) {
+    floatx16 s;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) s[e] = 0.0f;
+#pragma unroll
+    for (int j = 0; j < P; ++j) {
+      const intx8 k = {static_cast<int>(r.c[j][0]), static_cast<int>(r.c[j][1]),
+                       static_cast<int>(r.c[j][2]), static_cast<int>(r.c[j][3]), 0, 0, 0, 0};
+      const int scale = static_cast<int>(r.s[j]);  // 255: NaN
+      s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, q_lo[j], s, 4, 0, 0, scale, 1,
+                                                          q_scale[j]);
+      s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, q_hi[j], s, 4, 0, 0, scale, 0,
+                                                          q_scale[j]);
+    }
+    return s;
+  };
   // The prefix.  This wave's codes two tiles on are on their way; where it takes
   // every tile, its K one tile on (two sets of K registers did not fit: they spilled).
   auto products = [&](int t, auto parity) {  // of tile t, whose K is in rk[parity]
@@ -665,7 +692,7 @@ __device__ __forceinline__ void attn_unit_mx4(const SgTreeAttnMx4Args& args, Arg
                              static_cast<int64_t>(u.kv_head * G) * out_head;
   auto dst_of = [&](int q, int within) {
     const int mq = qg * 32 + q;
-    const int rq = mq / G;
+    const int rq = mq >> g_bits;
     return rq < u.row_count
                ? out_base + static_cast<int64_t>(rq) * out_row +
                      static_cast<int64_t>(mq - rq * G) * out_head + within / 2
