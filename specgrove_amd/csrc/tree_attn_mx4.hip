@@ -25,12 +25,14 @@
 // share a CU; streams are merged at the end.
 //
 // Measured (64 requests of 16,384 cached tokens, 32 q / 8 kv heads, d = 128; 1 / 16 /
-// 32 rows each): 243 / 432 / 644 us, that is 4.7 / 2.6 / 1.8 TB/s of codes and scales
-// and 71 / 636 / 854 TFLOP/s.  One row a request is bound by the cache's bytes, 32
-// by issue: a wave and tile take 124 vector instructions and 20 products.  Tried:
-// K and V unpacked to bf16 by the workgroup, 406 / 444 / 702; by each wave for
-// itself, 249 / 470 / 873; the products of a tile issued before the softmax of the
-// one before it, 583 / 381 / 672 (spills at one row).
+// 32 rows each): 238 / 362 / 612 us, that is 4.8 / 3.2 / 1.9 TB/s of codes and scales
+// and 72 / 759 / 898 TFLOP/s.  One row a request is bound by the cache's bytes, 32
+// by issue: a wave and tile take 124 vector instructions and 20 products, of which a
+// wave alone on its SIMD can overlap little (475 us for half the requests, one workgroup
+// a CU).  Tried: K and V unpacked to bf16 by the workgroup, 406 / 444 / 702; by each wave
+// for itself, 249 / 470 / 873; the products of a tile issued before the softmax of the
+// one before it, 583 / 381 / 672 (spills at one row); all of V read before the softmax,
+// 314 / 369 / 620; s_setprio around the products, no difference.
 #include <algorithm>
 #include <cmath>
 #include <map>
@@ -380,7 +382,9 @@ __device__ __forceinline__ void attn_unit_mx4(const SgTreeAttnMx4Args& args, Arg
       const short4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(at + 4 * ROWB));
       r.v[db] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     }
-    __builtin_amdgcn_sched_barrier(0);
+    // Keeps the reads here; in the private form that cost registers (268 against
+    // 238 us at one row).
+    if constexpr (kShared && !kBoth) __builtin_amdgcn_sched_barrier(0);
     return r;
   };
   // O^T += V^T P^T over half c.
@@ -767,8 +771,8 @@ struct UnitCost {
   double fixed[2];
   double window[2][4];
 };
-constexpr UnitCost kCost64 = {{6.0, 4.0}, {{0.55, 1.04, 1.84, 1.85}, {0.41, 0.89, 1.50, 1.56}}};
-constexpr UnitCost kCost128 = {{10.0, 8.0}, {{0.95, 1.69, 2.26, 2.51}, {0.72, 1.26, 1.75, 1.90}}};
+constexpr UnitCost kCost64 = {{6.0, 4.0}, {{0.49, 0.88, 1.82, 1.84}, {0.33, 0.67, 1.50, 1.55}}};
+constexpr UnitCost kCost128 = {{11.0, 7.0}, {{0.88, 1.35, 2.20, 2.33}, {0.63, 0.93, 1.70, 1.82}}};
 
 // The units of a wave by size: `count` of `micros` each.
 struct Alike {
