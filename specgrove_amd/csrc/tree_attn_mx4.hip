@@ -895,13 +895,22 @@ extern "C" int sg_tree_attn_plan_mx4(int32_t num_requests, const int32_t* row_of
                            static_cast<int64_t>(num_kv_heads) * (splits[i] - 1)});
       }
     }
-    for (const Alike& u : units) load += u.micros * u.count;
+    double largest = 0.0;
+    for (const Alike& u : units) {
+      load += u.micros * u.count;
+      largest = std::max(largest, u.micros);
+    }
+    const double merge = partial_bytes > 0.0 ? 12.0 + partial_bytes / 4.5e6 : 0.0;
+    // No cut ends before its mean load or its largest unit.
+    if (cut.share > 0.0 &&
+        merge + (alone ? largest : std::max(load / kSlots, 0.88 * largest)) >= best_end)
+      continue;
     // The units that start first, the largest, run at nearly the speed of one on the CU
     // (older waves issue first), and so do the last: seven eighths of the end at the
     // speed of two, but no less than the slots' mean load.
     double end = end_of(units, alone ? kDefaultCUs : kSlots);
     if (!alone) end = std::max(load / kSlots, 0.88 * end);
-    if (partial_bytes > 0.0) end += 12.0 + partial_bytes / 4.5e6;  // the merge
+    end += merge;
     if (cut.share == 0.0 || end < best_end) {
       best_end = end;
       wave.splits = splits;
