@@ -10,8 +10,10 @@
 // order as integers with infinities and NaNs above, so that those reach the scale.
 //
 // Bound by HBM: 16-byte loads, 8 values a lane; 16 lanes hold a block, so its
-// maximum takes four lane exchanges; 8-byte stores of codes.  Columns from K up to
-// the next multiple of 128 are written as zeros.
+// maximum takes four lane moves; 8-byte stores of codes.  Columns from K up to the
+// next multiple of 128 are written as zeros.  2048 rows: SiLU * up of 12288 columns
+// 27 us, 4.6 TB/s (39 with a division in the SiLU and exchanges through the LDS);
+// add + RMSNorm of 4096 with its sum 13 us, 4.5 TB/s.
 #include <algorithm>
 
 #include "sg_common.h"
@@ -53,9 +55,10 @@ __device__ __forceinline__ void store_block(const RowsOut& out, int64_t row, int
   uint32_t bits = 0u;
 #pragma unroll
   for (int k = 0; k < 8; ++k) bits = max(bits, __float_as_uint(x[k]) & 0x7fffffffu);
-#pragma unroll
-  for (int d = 1; d < 16; d <<= 1)
-    bits = max(bits, static_cast<uint32_t>(__shfl_xor(static_cast<int>(bits), d)));
+  bits = max(bits, lane_swap<kSwap1>(bits));
+  bits = max(bits, lane_swap<kSwap2>(bits));
+  bits = max(bits, lane_swap<kMirror8>(bits));
+  bits = max(bits, lane_swap<kMirror16>(bits));
   const float m = __uint_as_float(max(bits, kTinyBits));
   const float r = 448.0f / m;
   uint32_t w[2];

@@ -48,4 +48,14 @@ __device__ __forceinline__ uint16_t f32_to_bf16(float f) {
   return __builtin_bit_cast(uint16_t, static_cast<__bf16>(f));
 }
 
+// A value of another lane by a data-parallel move, no trip through the LDS: the lane
+// whose number differs in bit 0 (bit 1), and lane 7 - i of 8 (15 - i of 16), which
+// among lanes that agree in fours (eights) is as good as the other four (eight).
+constexpr int kSwap1 = 0xb1, kSwap2 = 0x4e, kMirror8 = 0x141, kMirror16 = 0x140;
+template <int kMove>
+__device__ __forceinline__ uint32_t lane_swap(uint32_t v) {
+  return static_cast<uint32_t>(
+      __builtin_amdgcn_mov_dpp(static_cast<int>(v), kMove, 0xf, 0xf, true));
+}
+
 }  // namespace sg
