@@ -751,8 +751,8 @@ extern "C" int sg_fp8_matmul(const SgFp8MatmulArgs* args, sg_stream_t stream) {
   SG_REQUIRE(a.codes_dev && a.scales_dev && a.weight_dev && a.weight_scales_dev && a.out_dev,
              "null device pointer");
   SG_REQUIRE(a.code_stride >= static_cast<int64_t>(steps) * 128 && a.code_stride % 16 == 0 &&
-                 a.code_stride < (int64_t{1} << 25),
-             "code_stride must be a multiple of 16 in [K padded to 128, 2^25)");
+                 a.code_stride <= (int64_t{1} << 24),  // 255 rows on: 32-bit offsets
+             "code_stride must be a multiple of 16 in [K padded to 128, 2^24]");
   SG_REQUIRE(a.scale_stride >= a.num_rows, "scale_stride must cover the rows");
   SG_REQUIRE(a.out_stride >= a.n && a.out_stride % 8 == 0,
              "out_stride must cover a row and be a multiple of 8");

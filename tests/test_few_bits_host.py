@@ -98,7 +98,7 @@ def _matmul(**fields):
     dict(num_rows=-1), dict(n=0), dict(k=0), dict(n=(1 << 24) + 1), dict(k=(1 << 24) + 1),
     dict(codes_dev=0), dict(scales_dev=0), dict(weight_dev=0), dict(weight_scales_dev=0),
     dict(out_dev=0), dict(scale_stride=3), dict(out_stride=248), dict(out_stride=260),
-    dict(code_stride=128), dict(codes_dev=264), dict(out_dev=264), dict(weight_dev=264)])
+    dict(code_stride=128), dict(code_stride=(1 << 24) + 16), dict(codes_dev=264), dict(out_dev=264), dict(weight_dev=264)])
 def test_matmul_refusals(fields):
     assert _matmul(**fields) == EINVAL
 
