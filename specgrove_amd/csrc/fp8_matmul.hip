@@ -543,25 +543,42 @@ __global__ __launch_bounds__(64 * KW) void fp8_matmul_few_kernel(MatmulArgs a) {
   // This wave's blocks are wave, wave + KW, ...
   const int mine = a.steps > wave ? (a.steps - wave + KW - 1) / KW : 0;
   auto block = [&](int k) { return wave + KW * k; };
-  Step now[kAhead], next[kAhead];
+  // Two sets of kAhead blocks take turns.  (One set copied into the other at the end of
+  // a turn made every turn wait for the loads it had issued.)
+  Step set[2][kAhead];
 #pragma unroll
   for (int u = 0; u < kAhead; ++u)
-    if (u < mine) load(block(u), now[u]);
+    if (u < mine) load(block(u), set[0][u]);
   int k = 0;
-  for (; k + 2 * kAhead <= mine; k += kAhead) {
+  auto turn = [&](auto parity) {  // of the blocks k .. in set[parity]
+    constexpr int p = decltype(parity)::value;
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) load(block(k + kAhead + u), next[u]);
+    for (int u = 0; u < kAhead; ++u) load(block(k + kAhead + u), set[1 - p][u]);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) multiply(now[u]);
+    for (int u = 0; u < kAhead; ++u) multiply(set[p][u]);
+    k += kAhead;
+  };
+  auto finish = [&](Step (&last)[kAhead]) {
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) now[u] = next[u];
+    for (int u = 0; u < kAhead; ++u)
+      if (k + u < mine) multiply(last[u]);
+    for (k += kAhead; k < mine; ++k) {
+      load(block(k), last[0]);
+      multiply(last[0]);
+    }
+  };
+  using Even = std::integral_constant<int, 0>;
+  using Odd = std::integral_constant<int, 1>;
+  while (k + 3 * kAhead <= mine) {
+    turn(Even{});
+    turn(Odd{});
   }
-#pragma unroll
-  for (int u = 0; u < kAhead; ++u)
-    if (k + u < mine) multiply(now[u]);
-  for (k += kAhead; k < mine; ++k) {
-    load(block(k), now[0]);
-    multiply(now[0]);
+  if (k + 2 * kAhead <= mine) {
+    turn(Even{});
+    finish(set[1]);
+  } else {
+    finish(set[0]);
   }
 
   if (KW > 1) {
@@ -652,7 +669,7 @@ __global__ __launch_bounds__(256) void fp8_pack_kernel(const unsigned char* __re
 }
 
 // How a call is cut: a kernel and the splits of K.
-enum Form { kFew1, kFew2, kFew2x2, kTile64, kTile64Pair, kTile128, kTile128Pair, kPp3, kPp4 };
+enum Form { kFew1, kFew2, kFew1x2, kFew2x2, kTile64, kTile64Pair, kTile128, kTile128Pair, kPp3, kPp4 };
 struct Cut {
   Form form;
   int splits;
@@ -660,9 +677,10 @@ struct Cut {
 
 // Rows up to 32 (up to 64 where the second pair of row blocks finds the weight in
 // L2, N <= 12,288) take the few-rows kernel: 64 rows of 4096 -> 4096 in 7.5 us, a
-// tile kernel 11.6; of 4096 -> 24576 in 31, a tile kernel 18.8.  One row block: two
-// weight blocks a wave once that leaves 160 workgroups (6144 x 2560 at 16 rows 4.4 us,
-// one block 5.2; 4096 x 12288 the other way round, 10.8 and 9.4).
+// tile kernel 11.6; of 4096 -> 24576 in 31, a tile kernel 18.8.  Two weight blocks a
+// wave once that leaves 160 workgroups (6144 x 2560 at 16 rows 4.4 us, one block 5.2;
+// at 32 rows 7.7 and 9.4; 4096 x 12288 the other way round, 10.8 and 9.4, at 32 rows
+// 21.2 and 18.5).
 //
 // Beyond, the tile kernels by an estimate: rounds of workgroups x blocks of K x
 // the time of a block (us, measured with every CU at work on 4096 -> 24576 and
@@ -676,7 +694,8 @@ struct Cut {
 // pairs 20.
 Cut cut_of(int rows, int n, int steps) {
   if (rows <= 16) return {n > 32 * 159 ? kFew2 : kFew1, 1};
-  if (rows <= 32 || (rows <= 64 && n <= 12288)) return {kFew2x2, 1};
+  if (rows <= 32 || (rows <= 64 && n <= 12288))
+    return {(n + 31) / 32 * ((rows + 31) / 32) < 160 ? kFew1x2 : kFew2x2, 1};
   struct Kind {
     Form form;
     int bn, bm, slots;  // workgroups at a time
@@ -800,6 +819,7 @@ extern "C" int sg_fp8_matmul(const SgFp8MatmulArgs* args, sg_stream_t stream) {
   switch (c.form) {
     case kFew1: launched = few(fp8_matmul_few_kernel<1, 1, 8>, 1, 1); break;
     case kFew2: launched = few(fp8_matmul_few_kernel<2, 1, 8>, 2, 1); break;
+    case kFew1x2: launched = few(fp8_matmul_few_kernel<1, 2, 8>, 1, 2); break;
     case kFew2x2: launched = few(fp8_matmul_few_kernel<2, 2, 8>, 2, 2); break;
     case kTile64: launched = go(fp8_matmul_kernel<128, 64, 2, 4, 6, 1>, 128, 64, 512); break;
     case kTile64Pair: launched = go(fp8_matmul_kernel<128, 64, 2, 2, 3, 2>, 128, 64, 256); break;
