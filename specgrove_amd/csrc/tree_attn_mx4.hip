@@ -807,8 +807,9 @@ double end_of(std::vector<Alike>& units, int64_t slots) {
 // what is fixed, and a long one holds the launch's end up as much: prefixes are cut so
 // that the estimated end of the last unit, and of the merge that pieces need, is earliest.
 // Against the bf16 plan, 32 q / 8 kv heads, d = 128: 32 requests of 8,192-32,768 tokens
-// and 1 to 64 rows 443 us (736); 7 of 16,307-32,614 and one row 51 (65); 7 of 524-1,048
-// and 1 to 64 rows 25 (29); 64 of 512-4,096 and 16 to 128 rows 94 (92).
+// and 1 to 64 rows 434 us (727); 7 of 16,307-32,614 and one row 50 (63); 7 of 524-1,048
+// and 1 to 64 rows 23 (28); 64 of 512-4,096 and 16 to 128 rows 86 (86); with 16 kv heads,
+// d = 64, 49 of 2,872-5,745 and 16 to 128 rows 95 (140).
 extern "C" int sg_tree_attn_plan_mx4(int32_t num_requests, const int32_t* row_offset_host,
                                      const int32_t* prefix_len_host, int32_t num_q_heads,
                                      int32_t num_kv_heads, int32_t head_dim, void* plan_host,
@@ -856,7 +857,8 @@ extern "C" int sg_tree_attn_plan_mx4(int32_t num_requests, const int32_t* row_of
     bool by_rows;
     double share;
   };
-  constexpr Cut kCuts[] = {{false, 0.0},  {true, 2.0},   {true, 1.4},  {true, 1.0},  {false, 2.0},
+  constexpr Cut kCuts[] = {{false, 0.0},  {true, 2.0},  {true, 1.6},
+                           {true, 1.4},   {true, 1.2},  {true, 1.0},  {false, 2.0},
                            {false, 1.6},  {false, 1.35}, {false, 1.15}, {false, 1.05}, {false, 0.8},
                            {false, 0.6}, {false, 0.45}, {false, 0.3}};
   for (const Cut& cut : kCuts) {
@@ -903,13 +905,18 @@ extern "C" int sg_tree_attn_plan_mx4(int32_t num_requests, const int32_t* row_of
     const double merge = partial_bytes > 0.0 ? 12.0 + partial_bytes / 4.5e6 : 0.0;
     // No cut ends before its mean load or its largest unit.
     if (cut.share > 0.0 &&
-        merge + (alone ? largest : std::max(load / kSlots, 0.88 * largest)) >= best_end)
+        merge + (alone ? largest : std::max(load / kSlots, 0.78 * largest)) >= best_end)
       continue;
-    // The units that start first, the largest, run at nearly the speed of one on the CU
-    // (older waves issue first), and so do the last: seven eighths of the end at the
-    // speed of two, but no less than the slots' mean load.
+    // A unit that starts at once and ends last has its CU to itself for the longer part
+    // (and older waves issue first): 0.68-0.83 of its time beside another one, measured;
+    // with a second turn of units on the slots, 0.84-0.96 of the end at the speed of two.
+    // The slots' mean load is passed by up to 0.15, less with smaller units or even loads.
     double end = end_of(units, alone ? kDefaultCUs : kSlots);
-    if (!alone) end = std::max(load / kSlots, 0.88 * end);
+    if (!alone && end > 0.0) {
+      const double grain = largest / end;
+      end = std::max(std::min(end, (1.0 + 0.15 * grain * grain) * load / kSlots),
+                     end > 1.001 * largest ? 0.93 * end : 0.78 * end);
+    }
     end += merge;
     if (cut.share == 0.0 || end < best_end) {
       best_end = end;
