@@ -25,8 +25,8 @@
 // share a CU; streams are merged at the end.
 //
 // Measured (64 requests of 16,384 cached tokens, 32 q / 8 kv heads, d = 128; 1 / 16 /
-// 32 rows each): 238 / 362 / 612 us, that is 4.8 / 3.2 / 1.9 TB/s of codes and scales
-// and 72 / 759 / 898 TFLOP/s.  One row a request is bound by the cache's bytes, 32
+// 32 rows each): 234 / 365 / 630 us, that is 4.9 / 3.1 / 1.8 TB/s of codes and scales
+// and 73 / 753 / 873 TFLOP/s.  One row a request is bound by the cache's bytes, 32
 // by issue: a wave and tile take 124 vector instructions and 20 products, of which a
 // wave alone on its SIMD can overlap little (475 us for half the requests, one workgroup
 // a CU).  Tried: K and V unpacked to bf16 by the workgroup, 406 / 444 / 702; by each wave
@@ -107,7 +107,7 @@ template <int D>
 struct Shared {
   static constexpr int kSlot = (2 + D / 2) * 64 * 4;   // a wave's state
   static constexpr int kStage = 32 * (2 * D + 16);     // a wave's output rows
-  static constexpr int kBytes = (kWaves - 1) * kSlot + kStage;
+  static constexpr int kBytes = kWaves * kSlot;
   static_assert(kBytes >= kWaves * kTileKeys * 2 * D && kBytes >= kSlot * 2 + kStage * 2 &&
                     kBytes >= kStage * 4,
                 "every use of the buffer must fit");
@@ -624,7 +624,73 @@ __device__ __forceinline__ void attn_unit_mx4(const SgTreeAttnMx4Args& args, Arg
   }
   __syncthreads();
 
-  // Merge the key streams of each q-group through LDS (the V tiles are done with).
+  if constexpr (!kShared) {
+    // The states of the q-group's four waves meet in LDS (the V tiles are done with);
+    // each of them merges a quarter of the columns and stores it.  (One wave for all of
+    // it, through a staging tile, took 4.5 us of a unit, issuing by itself.)
+    float* own = reinterpret_cast<float*>(sh.buf + wave * Shared<D>::kSlot);
+    own[lane] = st.m;
+    own[64 + lane] = st.l;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) own[(2 + 16 * db + r) * 64 + lane] = st.acc[db][r];
+    __syncthreads();
+    const float* slots =
+        reinterpret_cast<const float*>(sh.buf + qg * Shared<D>::kSlot) + lane;
+    constexpr int kNext = (kWaves / streams) * Shared<D>::kSlot / 4;  // the next stream's
+    float m_all = -__builtin_inff();
+#pragma unroll
+    for (int k = 0; k < streams; ++k) m_all = fmaxf(m_all, slots[k * kNext]);
+    const float m_use = (m_all == -__builtin_inff()) ? 0.0f : m_all;
+    float w[streams], l = 0.0f;
+#pragma unroll
+    for (int k = 0; k < streams; ++k) {
+      const float mk = slots[k * kNext];
+      w[k] = (mk == -__builtin_inff()) ? 0.0f : __builtin_amdgcn_exp2f((mk - m_use) * c2);
+      l += w[k] * slots[k * kNext + 64];
+    }
+    constexpr int kMine = 16 * DB / streams;  // of the 16 DB values of a lane
+    const int first = kMine * ks;
+    float o[kMine];
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      o[i] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < streams; ++k)
+        o[i] += w[k] * slots[k * kNext + (2 + first + i) * 64];
+    }
+    const ArgsIn z = fresh(in);
+    // Values 4 c .. 4 c + 3 of a lane are columns 8 c + 4 half .. + 3 of its query.
+    if (u.partial >= 0) {
+      // Layout: O as float4 chunks (2 c + half) * 128 + m, then the running max (log2
+      // units) and sum per query vector.
+      float* part = static_cast<float*>(z->attn.workspace_dev) + partial_floats(D) * u.partial;
+#pragma unroll
+      for (int c = 0; c < kMine / 4; ++c)
+        reinterpret_cast<float4*>(part)[(2 * (first / 4 + c) + half) * kQPerUnit + m] =
+            make_float4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
+      if (ks == 0 && half == 0) {
+        part[static_cast<size_t>(kQPerUnit) * D + m] = (m_all == -__builtin_inff()) ? m_all
+                                                                                    : m_all * c2;
+        part[static_cast<size_t>(kQPerUnit) * D + kQPerUnit + m] = l;
+      }
+      return;
+    }
+    if (r_local >= u.row_count) return;
+    const float inv = l > 0.0f ? 1.0f / l : l;  // NaN stays NaN
+    uint16_t* dst = static_cast<uint16_t*>(z->attn.out_dev) + row * z->attn.out_row_stride +
+                    static_cast<int64_t>(head) * z->attn.out_head_stride + 2 * first + 4 * half;
+#pragma unroll
+    for (int c = 0; c < kMine / 4; ++c)
+      *reinterpret_cast<uint2*>(dst + 8 * c) =
+          make_uint2(pack_bf16x2(o[4 * c] * inv, o[4 * c + 1] * inv),
+                     pack_bf16x2(o[4 * c + 2] * inv, o[4 * c + 3] * inv));
+    return;
+  }
+
+  // Merge the key streams of each q-group through LDS (done by one wave each:
+  // shared between both as above it measured the same).
   if (active && ks > 0) {
     float* slot = reinterpret_cast<float*>(sh.buf + ((ks - 1) * nq + qg) * Shared<D>::kSlot);
     slot[lane] = st.m;
