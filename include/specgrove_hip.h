@@ -472,7 +472,7 @@ typedef struct SgKvCommitMx4Args {
   int32_t num_layers;
   int32_t num_requests;
   int32_t num_kv_heads;
-  int32_t head_dim;                /* multiple of 32 */
+  int32_t head_dim;                /* multiple of 32; num_kv_heads * head_dim < 2^18 */
   /* per-layer bases of the arena (device arrays of num_layers device pointers) */
   void* const* k_code_layers_dev;
   void* const* k_scale_layers_dev;
@@ -573,7 +573,7 @@ typedef struct SgFp8MatmulArgs {
   int32_t k;                       /* columns of the activations */
   int32_t reserved;
   const void* codes_dev;           /* e4m3 [R, code_stride], 16-byte aligned */
-  int64_t code_stride;             /* multiple of 16, >= Kp */
+  int64_t code_stride;             /* multiple of 16 in [Kp, 2^24] */
   const float* scales_dev;         /* [Kp/128, scale_stride] */
   int64_t scale_stride;
   const void* weight_dev;          /* packed by sg_fp8_pack_weight */

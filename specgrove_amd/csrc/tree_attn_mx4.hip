@@ -161,8 +161,8 @@ __device__ __forceinline__ void attn_unit_mx4(const SgTreeAttnMx4Args& args, Arg
   const int g = u.kv_head;
   const bool do_tree = (u.flags & 1) != 0;
 
-  // What the start of the unit needs, loaded before the prefix's first codes: loads
-  // return in order, and one round trip serves all of it.
+  // The parents are on their way before the prefix's first codes: loads return in
+  // order.  (Q and the tree's first tile loaded here too spilled, and cost 3 us.)
   const int tree_keys = do_tree ? u.row_begin + u.row_count : 0;
   const int parent = do_tree ? load_parent(a, r0, n) : -1;
   // Q, bf16: piece [j][b][e] is columns 64 j + 32 b + 16 half + 8 e .. +7.
