@@ -138,6 +138,7 @@ class AttnPlan:
     head_dim: int
     device: torch.Tensor | None = None
     workspace: torch.Tensor | None = None
+    host_address: int = field(default=0, repr=False, compare=False)  # of host, once known
     # What the plan was made from, and the wave's plan over a 4-bit cache (in_mx4).
     wave: tuple | None = field(default=None, repr=False, compare=False)
     mx4: "AttnPlan | None" = field(default=None, repr=False, compare=False)
@@ -259,9 +260,11 @@ def check_plan_call(plan: AttnPlan, num_requests: int, num_rows: int, num_q_head
     _require((plan.num_q_heads, plan.num_kv_heads, plan.head_dim)
              == (num_q_heads, num_kv_heads, head_dim),
              "plan was built for another head configuration")
-    _require(plan.num_requests == num_requests and plan.num_rows == num_rows,
-             f"plan was built for another wave ({plan.num_requests} requests, "
-             f"{plan.num_rows} rows; the call has {num_requests} and {num_rows})")
+    header = plan.header
+    requests, packed = int(header[8]), int(header[9])
+    if requests != num_requests or packed != num_rows:
+        raise ValueError(f"plan was built for another wave ({requests} requests, {packed} rows; "
+                         f"the call has {num_requests} and {num_rows})")
 
 
 UNIT_FIELDS = ("req", "kv_head", "row_begin", "row_count", "key_begin", "key_end",
@@ -1020,6 +1023,8 @@ def _mx4_attention_args(q, k_codes, k_scales, v_codes, v_scales, k_tree, v_tree,
     _require(fits, "the arguments do not fit together")
     check_plan_call(plan, n, rows, hq, hkv, dim)
     plan = plan.in_mx4()
+    if plan.host_address == 0:
+        plan.host_address = plan.host.ctypes.data
     if out is None:
         out = torch.empty((rows, hq, dim), dtype=bf16, device=q.device)
     os = out.stride()
@@ -1029,7 +1034,7 @@ def _mx4_attention_args(q, k_codes, k_scales, v_codes, v_scales, k_tree, v_tree,
         at[0], qs[0], qs[1], at[1], at[2], cs[0], cs[1], at[3], at[4], ts[0], ts[1],
         row_offset.data_ptr(), prefix_start.data_ptr(), prefix_len.data_ptr(),
         parent.data_ptr(), out.data_ptr(), os[0], os[1],
-        plan.device.data_ptr(), plan.host.ctypes.data, plan.units, plan.merges,
+        plan.device.data_ptr(), plan.host_address, plan.units, plan.merges,
         workspace.data_ptr() if workspace is not None else 0,
         workspace.numel() if workspace is not None else 0,
         status.data_ptr() if status is not None else 0)
@@ -1086,7 +1091,8 @@ def prepare_kv_commit_mx4(k_code_ptrs: torch.Tensor, k_scale_ptrs: torch.Tensor,
              "request metadata sizes disagree")
     if status is not None:
         _check_device_tensor(status, "status", torch.int32)
-    _check_current(lengths, "lengths")
+    _check_current(lengths, "lengths", *pointers, prefix_start, row_offset, keep_len, keep_rows,
+                   status)
     a = _lib.SgKvCommitMx4Args(
         layers, n, num_kv_heads, head_dim, *(t.data_ptr() for t in pointers[:4]),
         code_head_stride, code_token_stride, scale_head_stride, scale_token_stride,
@@ -1122,7 +1128,7 @@ def kv_load_mx4(codes: torch.Tensor, scales: torch.Tensor,
     c, s, o = flat
     _require(not (c.data_ptr() | c.stride(0) | c.stride(1)) % 4,
              "codes must be 4-byte aligned, their strides multiples of 4 bytes")
-    _check_current(codes, "codes")
+    _check_current(codes, "codes", scales, out)
     _lib.check(_lib.load().sg_kv_load_mx4(
         c.data_ptr(), c.stride(0), c.stride(1), s.data_ptr(), s.stride(0), s.stride(1),
         c.shape[0], c.shape[1], dim, o.data_ptr(), o.stride(0), o.stride(1), _stream_handle()),
@@ -1162,9 +1168,14 @@ def _new_fp8_rows(rows: int, columns: int, device) -> "tuple[Fp8Rows, _lib.SgFp8
     return Fp8Rows(codes if padded == columns else codes[:, :columns], scales), out
 
 
-def _check_current(t: torch.Tensor, name: str) -> None:
-    if t.get_device() != torch.cuda.current_device():
+def _check_current(t: torch.Tensor, name: str, *others: torch.Tensor | None) -> None:
+    """t, and whatever else the call is given, on the current device."""
+    device = torch.cuda.current_device()
+    if t.get_device() != device:
         raise ValueError(f"{name} is on {t.device}, which is not the current device")
+    for o in others:
+        if o is not None and o.get_device() != device:
+            raise ValueError(f"a tensor is on {o.device}, {name} on {t.device}")
 
 
 def quantize_fp8(x: torch.Tensor) -> Fp8Rows:

@@ -107,7 +107,7 @@ def add_rmsnorm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float,
     if residual is not None:
         ops._check_rows(residual, "residual")
         ops._require(residual.shape == x.shape, "residual must be [R, H]")
-    ops._check_current(x, "x")
+    ops._check_current(x, "x", weight, residual)
     normed, out = ops._new_fp8_rows(rows, hidden, x.device)
     total = (torch.empty((rows, hidden), dtype=x.dtype, device=x.device) if want_sum else None)
     # Positional, in the order of SgAddRmsNormArgs' fields.

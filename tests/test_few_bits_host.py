@@ -239,3 +239,19 @@ def test_a_long_unit_is_cut_for_4_bits_and_refusals():
         with pytest.raises(ValueError):
             ops.plan_attention_mx4(*bad)
     assert ops.plan_attention_mx4([0], [], 32, 8, 128).units == 0
+
+
+def test_devices_are_compared(monkeypatch):
+    class On:
+        def __init__(self, index):
+            self.device = torch.device("cuda", index)
+
+        def get_device(self):
+            return self.device.index
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    ops._check_current(On(1), "x", On(1), None)
+    with pytest.raises(ValueError, match="not the current device"):
+        ops._check_current(On(0), "x")
+    with pytest.raises(ValueError, match="x on cuda:1"):
+        ops._check_current(On(1), "x", None, On(0))
