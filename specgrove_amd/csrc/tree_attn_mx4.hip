@@ -21,18 +21,19 @@
 // four key streams, each wave with V tiles of its own and no barrier; 2: two
 // streams; 3-4: one.  There the workgroup unpacks 64 keys of V at a time together,
 // a piece a thread, into one of two stages (one barrier for 64 keys).  Codes are
-// loaded two tiles (stages) ahead into registers: a tile is 4.3 KB.  Two workgroups
-// share a CU; streams are merged at the end.
+// loaded two tiles (stages) ahead into registers, K of 3-4 q-groups one tile: a tile is
+// 4.3 KB.  Two workgroups share a CU; streams are merged at the end.
 //
 // Measured (64 requests of 16,384 cached tokens, 32 q / 8 kv heads, d = 128; 1 / 16 /
 // 32 rows each): 234 / 365 / 630 us, that is 4.9 / 3.1 / 1.8 TB/s of codes and scales
 // and 73 / 753 / 873 TFLOP/s.  One row a request is bound by the cache's bytes, 32
-// by issue: a wave and tile take 124 vector instructions and 20 products, of which a
+// by issue: a wave and tile take 124 vector instructions and 12 products, of which a
 // wave alone on its SIMD can overlap little (475 us for half the requests, one workgroup
 // a CU).  Tried: K and V unpacked to bf16 by the workgroup, 406 / 444 / 702; by each wave
 // for itself, 249 / 470 / 873; the products of a tile issued before the softmax of the
 // one before it, 583 / 381 / 672 (spills at one row); all of V read before the softmax,
-// 314 / 369 / 620; s_setprio around the products, no difference.
+// 314 / 369 / 620; K two tiles ahead for 3-4 q-groups too (spills), 243 / 433 / 664;
+// s_setprio around the products, no difference.
 #include <algorithm>
 #include <cmath>
 #include <map>
