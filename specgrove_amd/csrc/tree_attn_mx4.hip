@@ -21,14 +21,15 @@
 // four key streams, each wave with V tiles of its own and no barrier; 2: two
 // streams; 3-4: one.  There the workgroup unpacks 64 keys of V at a time together,
 // a piece a thread, into one of two stages (one barrier for 64 keys).  Codes are
-// loaded two tiles (stages) ahead into registers, K of 3-4 q-groups one tile: a tile is
-// 4.3 KB.  Two workgroups share a CU; streams are merged at the end.
+// loaded two tiles (stages) ahead into registers: a tile is 4.3 KB.  K goes from there
+// into the products, for 3-4 q-groups through LDS, where all waves take it.  Two
+// workgroups share a CU; streams are merged at the end.
 //
 // Measured (64 requests of 16,384 cached tokens, 32 q / 8 kv heads, d = 128; 1 / 16 /
-// 32 rows each): 234 / 365 / 630 us, that is 4.9 / 3.1 / 1.8 TB/s of codes and scales
-// and 73 / 753 / 873 TFLOP/s.  One row a request is bound by the cache's bytes, 32
+// 32 rows each): 234 / 365 / 619 us, that is 4.9 / 3.1 / 1.8 TB/s of codes and scales
+// and 73 / 753 / 888 TFLOP/s.  One row a request is bound by the cache's bytes, 32
 // by issue: a wave and tile take 124 vector instructions and 12 products, of which a
-// wave alone on its SIMD can overlap little (475 us for half the requests, one workgroup
+// wave alone on its SIMD can overlap little (450 us for half the requests, one workgroup
 // a CU).  Tried: K and V unpacked to bf16 by the workgroup, 406 / 444 / 702; by each wave
 // for itself, 249 / 470 / 873; the products of a tile issued before the softmax of the
 // one before it, 583 / 381 / 672 (spills at one row); all of V read before the softmax,
@@ -60,6 +61,10 @@ __device__ __forceinline__ bf16x2 as_pair(uint32_t w) { return __builtin_bit_cas
 // chunk of each block of four (two) consecutive rows: the low bits.  (4 (r & 3) +
 // 2 (r >> 1 & 1), right for the reads alone, spent half of the LDS's active cycles
 // on conflicts of the writes.)  Both repeat every four rows.
+template <int D>
+__host__ __device__ constexpr int swz_kc(int r) {  // of K's codes: 16 rows at one chunk
+  return D == 128 ? (r >> 2) & 3 : (r >> 3) & 1;
+}
 template <int D>
 __host__ __device__ constexpr int swz_w(int r) {
   return D == 128 ? 5 * (r & 3) : 5 * ((r >> 1) & 1);
@@ -258,11 +263,11 @@ __device__ __forceinline__ void attn_unit_mx4(const SgTreeAttnMx4Args& args, Arg
     }
   };
   // Tile t's V (private), window t's piece of this thread (shared).
-  auto load_v = [&](int t, Raw& r) {
+  auto load_rows = [&](GlobalBytes codes, GlobalBytes scales, int t, Raw& r) {
     constexpr int kKeys = kShared ? kWindow : kTileKeys;
     if (kShared && !w_piece) return;
-    const GlobalBytes c = v_codes + static_cast<int64_t>(t) * kKeys * c_stride;
-    const GlobalBytes s = v_scales + static_cast<int64_t>(t) * kKeys * s_stride;
+    const GlobalBytes c = codes + static_cast<int64_t>(t) * kKeys * c_stride;
+    const GlobalBytes s = scales + static_cast<int64_t>(t) * kKeys * s_stride;
     const int last = prefix_keys - 1 - t * kKeys;
 #pragma unroll
     for (int i = 0; i < (kShared ? 1 : P); ++i) {
@@ -276,11 +281,18 @@ __device__ __forceinline__ void attn_unit_mx4(const SgTreeAttnMx4Args& args, Arg
       r.s[i] = s[sa];
     }
   };
+  auto load_v = [&](int t, Raw& r) { load_rows(v_codes, v_scales, t, r); };
+  auto load_kw = [&](int w, Raw& r) { load_rows(k_codes, k_scales, w, r); };  // a window's K
   // rk[p], rv[p]: this wave's tiles (windows) of even (odd) number.
   const int windows = (prefix_keys + kWindow - 1) / kWindow;
   Raw rk[2], rv[2];
-  if (ks < tiles) load_k(ks, rk[0]);
-  if (!kBoth && ks + streams < tiles) load_k(ks + streams, rk[1]);
+  if constexpr (kBoth) {
+    if (windows > 0) load_kw(0, rk[0]);
+    if (windows > 1) load_kw(1, rk[1]);
+  } else {
+    if (ks < tiles) load_k(ks, rk[0]);
+    if (ks + streams < tiles) load_k(ks + streams, rk[1]);
+  }
   if constexpr (kShared) {
     if (windows > 0) load_v(0, rv[0]);
     if (windows > 1) load_v(1, rv[1]);
@@ -339,6 +351,37 @@ __device__ __forceinline__ void attn_unit_mx4(const SgTreeAttnMx4Args& args, Arg
     for (int c = 0; c < 4; ++c)
       *reinterpret_cast<uint4*>(sh.buf + p * kWindow * ROWB + (w_at ^ (16 * c))) =
           unpack8(w[c], scale);
+  };
+  // Where every wave takes every tile (kBoth), the workgroup brings K into LDS too, as it
+  // is held, each thread a piece: waves that loaded whole tiles for themselves had
+  // registers for one tile ahead only (16,384 tokens, 32 rows: 631 us, 619 so; with two
+  // q-groups it lost, 368 and 410).  K of a window lies behind V's stages: rows of D / 2 bytes whose 16-byte chunk c
+  // is at c ^ swz_kc(row), then the scales.
+  constexpr int kRowK = D / 2;
+  constexpr int kStageK = kWindow * (kRowK + kBlocks);
+  unsigned char* const s_k = sh.buf + 2 * kWindow * ROWB;
+  static_assert(2 * kWindow * ROWB + 2 * kStageK <= Shared<D>::kBytes, "K's stages must fit");
+  auto put_k = [&](const Raw& r, int p) {
+    if (!w_piece) return;
+    unsigned char* st = s_k + p * kStageK;
+    *reinterpret_cast<u32x4*>(st + w_row * kRowK + 16 * (v_blk ^ swz_kc<D>(w_row))) = r.c[0];
+    st[kWindow * kRowK + w_row * kBlocks + v_blk] = static_cast<unsigned char>(r.s[0]);
+  };
+  // This lane's operands of tile i of stage p.
+  auto take_k = [&](int p, int i) {
+    const unsigned char* st = s_k + p * kStageK;
+    const int row = kTileKeys * i + k_key;
+    Raw r;
+#pragma unroll
+    for (int j = 0; j < P; ++j)
+      r.c[j] = *reinterpret_cast<const u32x4*>(st + row * kRowK +
+                                               16 * ((2 * j + half) ^ swz_kc<D>(row)));
+    const unsigned char* sc = st + kWindow * kRowK + row * kBlocks;
+    const uint32_t all = D == 128 ? *reinterpret_cast<const uint32_t*>(sc)
+                                  : *reinterpret_cast<const uint16_t*>(sc);
+#pragma unroll
+    for (int j = 0; j < P; ++j) r.s[j] = (all >> (8 * half + 16 * j)) & 0xffu;
+    return r;
   };
   // Online softmax of the tile's scores x (masked already): probabilities in x.
   // The reference point st.m moves only when a lane's maximum grew by more than
@@ -537,13 +580,11 @@ __device__ __forceinline__ void attn_unit_mx4(const SgTreeAttnMx4Args& args, Arg
     }
     return s;
   };
-  // The prefix.  This wave's codes two tiles on are on their way; where it takes
-  // every tile, its K one tile on (two sets of K registers did not fit: they spilled).
+  // The prefix.  This wave's codes two tiles (windows) on are on their way.
   auto products = [&](int t, auto parity) {  // of tile t, whose K is in rk[parity]
     constexpr int p = decltype(parity)::value;
-    constexpr int kAhead = kBoth ? 1 : 2;
     const floatx16 s = qk(rk[p]);
-    if (t + kAhead * streams < tiles) load_k(t + kAhead * streams, rk[p]);
+    if (t + 2 * streams < tiles) load_k(t + 2 * streams, rk[p]);
     return s;
   };
   auto attend = [&](floatx16 x, int t, const unsigned char* v0) {
@@ -569,23 +610,31 @@ __device__ __forceinline__ void attn_unit_mx4(const SgTreeAttnMx4Args& args, Arg
       constexpr int p = decltype(parity)::value;
       __syncthreads();  // stage p is whole, the other one read
       if (w + 1 < windows) {
+        if constexpr (kBoth) put_k(rk[1 - p], 1 - p);
         put_w(rv[1 - p], 1 - p);
-        if (w + 3 < windows) load_v(w + 3, rv[1 - p]);
+        if (w + 3 < windows) {
+          if constexpr (kBoth) load_kw(w + 3, rk[1 - p]);
+          load_v(w + 3, rv[1 - p]);
+        }
       }
       const unsigned char* v0 = sh.buf + p * kWindow * ROWB;
       if constexpr (kBoth) {
         if (!active) return;
-        attend(products(2 * w, Even{}), 2 * w, v0);
+        attend(qk(take_k(p, 0)), 2 * w, v0);
         if (2 * w + 1 >= tiles) return;
-        attend(products(2 * w + 1, Even{}), 2 * w + 1, v0 + kTileKeys * ROWB);
+        attend(qk(take_k(p, 1)), 2 * w + 1, v0 + kTileKeys * ROWB);
       } else {
         const int t = 2 * w + ks;
         if (t < tiles) attend(products(t, parity), t, v0 + ks * kTileKeys * ROWB);
       }
     };
     if (windows > 0) {
+      if constexpr (kBoth) put_k(rk[0], 0);
       put_w(rv[0], 0);
-      if (windows > 2) load_v(2, rv[0]);
+      if (windows > 2) {
+        if constexpr (kBoth) load_kw(2, rk[0]);
+        load_v(2, rv[0]);
+      }
     }
     for (int w = 0; w < windows; w += 2) {
       window(w, Even{});
@@ -838,8 +887,8 @@ struct UnitCost {
   double fixed[2];
   double window[2][4];
 };
-constexpr UnitCost kCost64 = {{6.0, 4.0}, {{0.49, 0.88, 1.82, 1.84}, {0.33, 0.67, 1.50, 1.55}}};
-constexpr UnitCost kCost128 = {{11.0, 7.0}, {{0.88, 1.35, 2.20, 2.33}, {0.63, 0.93, 1.70, 1.82}}};
+constexpr UnitCost kCost64 = {{6.0, 4.0}, {{0.49, 0.88, 1.48, 1.50}, {0.33, 0.67, 1.00, 1.03}}};
+constexpr UnitCost kCost128 = {{11.0, 7.0}, {{0.88, 1.35, 2.20, 2.33}, {0.63, 0.93, 1.62, 1.74}}};
 
 // The units of a wave by size: `count` of `micros` each.
 struct Alike {
@@ -874,9 +923,9 @@ double end_of(std::vector<Alike>& units, int64_t slots) {
 // what is fixed, and a long one holds the launch's end up as much: prefixes are cut so
 // that the estimated end of the last unit, and of the merge that pieces need, is earliest.
 // Against the bf16 plan, 32 q / 8 kv heads, d = 128: 32 requests of 8,192-32,768 tokens
-// and 1 to 64 rows 434 us (727); 7 of 16,307-32,614 and one row 50 (63); 7 of 524-1,048
-// and 1 to 64 rows 23 (28); 64 of 512-4,096 and 16 to 128 rows 86 (86); with 16 kv heads,
-// d = 64, 49 of 2,872-5,745 and 16 to 128 rows 95 (140).
+// and 1 to 64 rows 436 us (693); 7 of 16,307-32,614 and one row 50 (63); 7 of 524-1,048
+// and 1 to 64 rows 22 (28); 64 of 512-4,096 and 16 to 128 rows 89 (89); d = 64, 2 of
+// 27,218 and 256 rows 163 (235).
 extern "C" int sg_tree_attn_plan_mx4(int32_t num_requests, const int32_t* row_offset_host,
                                      const int32_t* prefix_len_host, int32_t num_q_heads,
                                      int32_t num_kv_heads, int32_t head_dim, void* plan_host,
