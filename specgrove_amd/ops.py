@@ -141,7 +141,8 @@ class AttnPlan:
     host_address: int = field(default=0, repr=False, compare=False)  # of host, once known
     # What the plan was made from, and the wave's plan over a 4-bit cache (in_mx4).
     wave: tuple | None = field(default=None, repr=False, compare=False)
-    mx4: "AttnPlan | None" = field(default=None, repr=False, compare=False)
+    # (No copy by dataclasses.replace carries it: its memory is not the copy's.)
+    mx4: "AttnPlan | None" = field(default=None, init=False, repr=False, compare=False)
 
     @property
     def header(self) -> np.ndarray:
@@ -163,24 +164,29 @@ class AttnPlan:
         self.device = torch.from_numpy(self.host).to(device, non_blocking=False)
         self.workspace = torch.zeros(max(self.workspace_bytes, 16), dtype=torch.uint8,
                                      device=device)
+        self.mx4 = None  # of the device before
         return self
 
     def with_workspace(self) -> "AttnPlan":
         """The same plan on the device with a workspace of its own, of the
         current stream's memory: calls that can overlap, as on two streams,
         must not share one."""
-        return replace(self, workspace=torch.empty(
-            max(self.workspace_bytes, 16), dtype=torch.uint8, device=self.device.device),
-            mx4=self.mx4.with_workspace() if self.mx4 is not None else None)
+        plan = replace(self, workspace=torch.empty(
+            max(self.workspace_bytes, 16), dtype=torch.uint8, device=self.device.device))
+        if self.mx4 is not None and self.mx4.device.device == self.device.device:
+            plan.mx4 = self.mx4.with_workspace()
+        return plan
 
     def in_mx4(self) -> "AttnPlan":
         """The plan that ``tree_attention_mx4`` runs of this one: itself if it was made
         for a 4-bit cache or a given number of units, else ``plan_attention_mx4`` of the
-        same wave, made and copied at the first use and kept (not while a stream is
-        captured: use the plan once before)."""
+        same wave, made and copied at the first use on a device and kept (not while a
+        stream is captured: use the plan once before).  Its workspace is memory of the
+        stream of that first use; another stream takes a ``with_workspace()`` of the plan."""
         if self.wave is None:
             return self
-        if self.mx4 is None:
+        if self.mx4 is None or self.mx4.device.device != self.device.device:
+            check_plan(self, *self.wave)  # the host copy may have been replaced
             _require(not torch.cuda.is_current_stream_capturing(),
                      "the plan's 4-bit form is made at its first use: call once before a "
                      "capture, or use plan_attention_mx4")
