@@ -370,8 +370,9 @@ def prepare_tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
         workspace.data_ptr() if workspace is not None else 0,
         workspace.numel() if workspace is not None else 0,
         status.data_ptr() if status is not None else 0)
+    # The plan's tensors too: the plan may be moved and then holds others.
     keep = (q, k_cache, v_cache, k_tree, v_tree, row_offset, prefix_start, prefix_len, parent,
-            plan, out, status)
+            plan.device, plan.host, workspace, out, status)
     return PreparedCall("sg_tree_attn_fwd", a, keep, result=out)
 
 
@@ -907,9 +908,9 @@ def tree_attention_mx4(q: torch.Tensor, k_codes: torch.Tensor, k_scales: torch.T
                        status: torch.Tensor | None = None) -> torch.Tensor:
     """Packed tree attention of one layer over a 4-bit cache (see
     prepare_tree_attention_mx4)."""
-    args, out = _mx4_attention_args(q, k_codes, k_scales, v_codes, v_scales, k_tree, v_tree,
-                                    row_offset, prefix_start, prefix_len, parent, plan, out,
-                                    scale, status)
+    args, out, _ = _mx4_attention_args(q, k_codes, k_scales, v_codes, v_scales, k_tree, v_tree,
+                                       row_offset, prefix_start, prefix_len, parent, plan, out,
+                                       scale, status)
     _lib.check(_lib.load().sg_tree_attn_mx4_fwd(ctypes.byref(args), _stream_handle()),
                "sg_tree_attn_mx4_fwd")
     return out
@@ -931,11 +932,11 @@ def prepare_tree_attention_mx4(q: torch.Tensor, k_codes: torch.Tensor, k_scales:
     last token is not looked at.  An infinity or a NaN in a tree row reaches only
     the rows that see it; a cached row packed from one gives NaN.
     """
-    args, out = _mx4_attention_args(q, k_codes, k_scales, v_codes, v_scales, k_tree, v_tree,
-                                    row_offset, prefix_start, prefix_len, parent, plan, out,
-                                    scale, status)
+    args, out, run = _mx4_attention_args(q, k_codes, k_scales, v_codes, v_scales, k_tree, v_tree,
+                                         row_offset, prefix_start, prefix_len, parent, plan, out,
+                                         scale, status)
     keep = (q, k_codes, k_scales, v_codes, v_scales, k_tree, v_tree, row_offset, prefix_start,
-            prefix_len, parent, plan, out, status)
+            prefix_len, parent, run.device, run.host, run.workspace, out, status)
     return PreparedCall("sg_tree_attn_mx4_fwd", args, keep, result=out)
 
 
@@ -984,7 +985,8 @@ def _explain_mx4_attention(q, k_codes, k_scales, v_codes, v_scales, k_tree, v_tr
 
 def _mx4_attention_args(q, k_codes, k_scales, v_codes, v_scales, k_tree, v_tree, row_offset,
                         prefix_start, prefix_len, parent, plan, out, scale, status):
-    """The call's argument struct and output, of arguments that fit.
+    """The call's argument struct and output, of arguments that fit, and the plan that
+    it runs.
 
     A call takes a few microseconds on the GPU at the least, so everything is
     looked at once here; what is wrong is found out by _explain_mx4_attention."""
@@ -1045,7 +1047,7 @@ def _mx4_attention_args(q, k_codes, k_scales, v_codes, v_scales, k_tree, v_tree,
         workspace.numel() if workspace is not None else 0,
         status.data_ptr() if status is not None else 0)
     return _lib.SgTreeAttnMx4Args(attn, k_scales.data_ptr(), v_scales.data_ptr(), ss[0],
-                                  ss[1]), out
+                                  ss[1]), out, plan
 
 
 def kv_commit_mx4(k_code_ptrs: torch.Tensor, k_scale_ptrs: torch.Tensor,

@@ -1,7 +1,10 @@
 """Where a plan's tensors live and who keeps them, on the CPU: CPU and meta tensors stand
 for two devices, and nothing is launched."""
 import dataclasses
+import gc
+import weakref
 
+import numpy as np
 import pytest
 import torch
 
@@ -55,3 +58,40 @@ def test_the_4_bit_form_is_of_the_plans_own_wave():
     mixed = dataclasses.replace(plan, host=other.host)
     with pytest.raises(ValueError):
         mixed.in_mx4()
+
+
+def _meta_tensors(offset, lengths):
+    parents = [k - 1 for n in np.diff(offset) for k in range(n)]
+    return [torch.from_numpy(np.asarray(a, t)) for a, t in (
+        (offset, np.int32), (np.zeros(len(lengths)), np.int64), (lengths, np.int32),
+        (parents, np.int32))]
+
+
+def _call(plan, **kw):
+    """A bound call over small CPU tensors (nothing is launched)."""
+    rows = WAVE[0][-1]
+    q = torch.zeros((rows, 32, 128), dtype=torch.bfloat16)
+    tree = torch.zeros((2, rows, 8, 128), dtype=torch.bfloat16)
+    codes = torch.zeros((8, 64, 64), dtype=torch.uint8)
+    scales = torch.zeros((8, 64, 4), dtype=torch.uint8)
+    return ops.prepare_tree_attention_mx4(q, codes, scales, codes, scales, *tree,
+                                          *_meta_tensors(*WAVE), plan, **kw)
+
+
+@pytest.mark.parametrize("make", [ops.plan_attention, ops.plan_attention_mx4])
+def test_a_prepared_call_keeps_the_plans_memory(make):
+    plan = make(*WAVE, 32, 8, 128).to("cpu")
+    call = _call(plan)
+    run = plan.in_mx4()
+    attn = call._args.attn
+    assert attn.plan_dev == run.device.data_ptr() and attn.workspace_dev
+    held = {"plan_dev": weakref.ref(run.device), "workspace_dev": weakref.ref(run.workspace),
+            "plan_host": weakref.ref(run.host)}
+    plan.to("meta")
+    plan.host = np.zeros_like(plan.host)
+    del run, plan
+    gc.collect()
+    assert all(ref() is not None for ref in held.values()), held
+    assert held["plan_dev"]().data_ptr() == attn.plan_dev
+    assert held["workspace_dev"]().data_ptr() == attn.workspace_dev
+    assert held["plan_host"]().ctypes.data == attn.plan_host
