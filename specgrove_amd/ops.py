@@ -138,7 +138,6 @@ class AttnPlan:
     head_dim: int
     device: torch.Tensor | None = None
     workspace: torch.Tensor | None = None
-    host_address: int = field(default=0, repr=False, compare=False)  # of host, once known
     # What the plan was made from, and the wave's plan over a 4-bit cache (in_mx4).
     wave: tuple | None = field(default=None, repr=False, compare=False)
     # (No copy by dataclasses.replace carries it: its memory is not the copy's.)
@@ -1031,8 +1030,6 @@ def _mx4_attention_args(q, k_codes, k_scales, v_codes, v_scales, k_tree, v_tree,
     _require(fits, "the arguments do not fit together")
     check_plan_call(plan, n, rows, hq, hkv, dim)
     plan = plan.in_mx4()
-    if plan.host_address == 0:
-        plan.host_address = plan.host.ctypes.data
     if out is None:
         out = torch.empty((rows, hq, dim), dtype=bf16, device=q.device)
     os = out.stride()
@@ -1042,7 +1039,7 @@ def _mx4_attention_args(q, k_codes, k_scales, v_codes, v_scales, k_tree, v_tree,
         at[0], qs[0], qs[1], at[1], at[2], cs[0], cs[1], at[3], at[4], ts[0], ts[1],
         row_offset.data_ptr(), prefix_start.data_ptr(), prefix_len.data_ptr(),
         parent.data_ptr(), out.data_ptr(), os[0], os[1],
-        plan.device.data_ptr(), plan.host_address, plan.units, plan.merges,
+        plan.device.data_ptr(), plan.host.ctypes.data, plan.units, plan.merges,
         workspace.data_ptr() if workspace is not None else 0,
         workspace.numel() if workspace is not None else 0,
         status.data_ptr() if status is not None else 0)

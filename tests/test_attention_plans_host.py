@@ -1,7 +1,9 @@
 """Where a plan's tensors live and who keeps them, on the CPU: CPU and meta tensors stand
 for two devices, and nothing is launched."""
+import copy
 import dataclasses
 import gc
+import pickle
 import weakref
 
 import numpy as np
@@ -95,3 +97,20 @@ def test_a_prepared_call_keeps_the_plans_memory(make):
     assert held["plan_dev"]().data_ptr() == attn.plan_dev
     assert held["workspace_dev"]().data_ptr() == attn.workspace_dev
     assert held["plan_host"]().ctypes.data == attn.plan_host
+
+
+@pytest.mark.parametrize("how", ["deepcopy", "pickle", "replace", "assigned"])
+@pytest.mark.parametrize("make", [ops.plan_attention, ops.plan_attention_mx4])
+def test_copies_of_a_used_plan_read_their_own_host_records(make, how):
+    plan = make(*WAVE, 32, 8, 128).to("cpu")
+    _call(plan)
+    if how == "deepcopy":
+        other = copy.deepcopy(plan)
+    elif how == "pickle":
+        other = pickle.loads(pickle.dumps(plan))
+    elif how == "replace":
+        other = dataclasses.replace(plan, host=plan.host.copy())
+    else:
+        other = plan
+        plan.host = plan.host.copy()
+    assert _call(other)._args.attn.plan_host == other.in_mx4().host.ctypes.data
