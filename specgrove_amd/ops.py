@@ -999,8 +999,16 @@ def _mx4_attention_args(q, k_codes, k_scales, v_codes, v_scales, k_tree, v_tree,
         n = prefix_len.numel()
         device = q.get_device()  # -1 on the CPU
         kv = (hkv, tokens, half // 16)
+        fits = True
+        if out is not None:
+            os = out.stride()
+            fits = (out.dtype == bf16 and out.shape == q.shape and os[2] == 1
+                    and not (os[0] | os[1]) & 7 and not out.data_ptr() & 15
+                    and out.get_device() == device)
+        if status is not None:
+            fits = fits and status.dtype == i32 and status.get_device() == device
         fits = (
-            q.dtype == bf16 and k_tree.dtype == bf16 and v_tree.dtype == bf16
+            fits and q.dtype == bf16 and k_tree.dtype == bf16 and v_tree.dtype == bf16
             and k_codes.dtype == u8 and k_scales.dtype == u8 and v_codes.dtype == u8
             and v_scales.dtype == u8 and row_offset.dtype == i32 and prefix_len.dtype == i32
             and parent.dtype == i32 and prefix_start.dtype == torch.int64
@@ -1024,7 +1032,7 @@ def _mx4_attention_args(q, k_codes, k_scales, v_codes, v_scales, k_tree, v_tree,
             and plan.device is not None and plan.device.get_device() == device)
     except (AttributeError, TypeError, ValueError, RuntimeError):  # no tensors, no GPU
         fits = False
-    if not fits or out is not None or status is not None:
+    if not fits:
         _explain_mx4_attention(q, k_codes, k_scales, v_codes, v_scales, k_tree, v_tree,
                                row_offset, prefix_start, prefix_len, parent, plan, out, status)
     _require(fits, "the arguments do not fit together")
@@ -1032,7 +1040,7 @@ def _mx4_attention_args(q, k_codes, k_scales, v_codes, v_scales, k_tree, v_tree,
     plan = plan.in_mx4()
     if out is None:
         out = torch.empty((rows, hq, dim), dtype=bf16, device=q.device)
-    os = out.stride()
+        os = out.stride()
     workspace = plan.workspace
     attn = _lib.SgTreeAttnArgs(
         n, rows, hq, hkv, dim, float(dim ** -0.5 if scale is None else scale),

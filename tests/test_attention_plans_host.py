@@ -114,3 +114,28 @@ def test_copies_of_a_used_plan_read_their_own_host_records(make, how):
         other = plan
         plan.host = plan.host.copy()
     assert _call(other)._args.attn.plan_host == other.in_mx4().host.ctypes.data
+
+
+def test_arguments_that_fit_are_looked_at_once(monkeypatch):
+    """The check of one argument at a time is for calls that do not fit, an output or a
+    status word given or not: it took longer than the call it stands before."""
+    def explain(*args):
+        raise AssertionError("looked at again")
+
+    plan = ops.plan_attention_mx4(*WAVE, 32, 8, 128).to("cpu")
+    out = torch.zeros((2, 32, 128), dtype=torch.bfloat16)
+    status = torch.zeros(1, dtype=torch.int32)
+    with monkeypatch.context() as patched:
+        patched.setattr(ops, "_explain_mx4_attention", explain)
+        for kw in ({}, dict(out=out), dict(status=status), dict(out=out, status=status)):
+            call = _call(plan, **kw)
+            assert call._args.attn.status_dev == (status.data_ptr() if "status" in kw else None)
+            assert (call.result is out) == ("out" in kw)
+    wide = torch.zeros((2, 32, 136), dtype=torch.bfloat16)
+    assert _call(plan, out=wide[:, :, :128])._args.attn.out_head_stride == 136
+    for bad in (dict(out=out.float()), dict(out=out[:1]), dict(out=out.transpose(0, 1)),
+                dict(out=torch.zeros((2, 32, 132), dtype=torch.bfloat16)[:, :, :128]),
+                dict(out=wide[:, :, 4:132]), dict(out=out.to("meta")[:, :1]),
+                dict(status=status.long()), dict(out=[1]), dict(status=1)):
+        with pytest.raises(ValueError):
+            _call(plan, **bad)
