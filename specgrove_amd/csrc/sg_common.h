@@ -4,6 +4,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <exception>
+#include <new>
 #include <string>
 
 #include "specgrove_hip.h"
@@ -26,6 +28,19 @@ void clear_error();
       return ::sg::set_error(SG_EHIP, std::string(#expr) + ": " +            \
                                           hipGetErrorString(sg_err_));       \
   } while (0)
+
+// The host work of a C entry: no exception leaves the entry.  (The first message is
+// short enough to need no memory.)
+template <class Work>
+int guarded(Work&& work) {
+  try {
+    return work();
+  } catch (const std::bad_alloc&) {
+    return set_error(SG_EHIP, "no host memory");
+  } catch (const std::exception& e) {
+    return set_error(SG_EHIP, e.what());
+  }
+}
 
 // Launch check: reports the launch error of the last kernel on this thread.
 #define SG_LAUNCH_CHECK() SG_HIP_CHECK(hipGetLastError())

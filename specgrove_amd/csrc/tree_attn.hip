@@ -1066,23 +1066,14 @@ int emit_plan(const PlanWave& w, const PlanOut& out) {
   return SG_OK;
 }
 
-}  // namespace sg
+namespace {
 
-extern "C" int sg_tree_attn_plan(int32_t num_requests, const int32_t* row_offset_host,
-                                 const int32_t* prefix_len_host, int32_t num_q_heads,
-                                 int32_t num_kv_heads, int32_t head_dim,
-                                 int32_t target_units_hint, void* plan_host,
-                                 size_t plan_capacity_bytes, size_t* plan_bytes,
-                                 int32_t* plan_units, int32_t* plan_merges,
-                                 size_t* workspace_bytes) {
-  using namespace sg;
-  clear_error();
-  PlanWave wave = {num_requests, row_offset_host, prefix_len_host, num_q_heads, num_kv_heads,
-                   head_dim};
-  const PlanOut out = {plan_host,  plan_capacity_bytes, plan_bytes,
-                       plan_units, plan_merges,         workspace_bytes};
+int plan_bf16(PlanWave wave, const PlanOut& out, int32_t target_units_hint) {
   if (const int rc = check_plan_wave(wave, out)) return rc;
-  const int G = num_q_heads / num_kv_heads;
+  const int num_requests = wave.num_requests, num_kv_heads = wave.num_kv_heads;
+  const int32_t* const row_offset_host = wave.row_offset;
+  const int32_t* const prefix_len_host = wave.prefix_len;
+  const int G = wave.num_q_heads / num_kv_heads;
   const int rows_per_tile = kQPerUnit / G;
 
   // Units of one (request, kv head, row tile) are split over their prefix when
@@ -1183,6 +1174,25 @@ extern "C" int sg_tree_attn_plan(int32_t num_requests, const int32_t* row_offset
                                                        prefix_len_host[i] / (4 * kTileKeys)));
   }
   return emit_plan(wave, out);
+}
+
+}  // namespace
+}  // namespace sg
+
+extern "C" int sg_tree_attn_plan(int32_t num_requests, const int32_t* row_offset_host,
+                                 const int32_t* prefix_len_host, int32_t num_q_heads,
+                                 int32_t num_kv_heads, int32_t head_dim,
+                                 int32_t target_units_hint, void* plan_host,
+                                 size_t plan_capacity_bytes, size_t* plan_bytes,
+                                 int32_t* plan_units, int32_t* plan_merges,
+                                 size_t* workspace_bytes) {
+  using namespace sg;
+  clear_error();
+  const PlanWave wave = {num_requests, row_offset_host, prefix_len_host,
+                         num_q_heads,  num_kv_heads,    head_dim};
+  const PlanOut out = {plan_host,  plan_capacity_bytes, plan_bytes,
+                       plan_units, plan_merges,         workspace_bytes};
+  return guarded([&] { return plan_bf16(wave, out, target_units_hint); });
 }
 
 extern "C" int sg_tree_attn_plan_check(const void* plan_host, int32_t num_requests,

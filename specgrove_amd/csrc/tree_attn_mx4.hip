@@ -916,9 +916,6 @@ double end_of(std::vector<Alike>& units, int64_t slots) {
   return end;
 }
 
-}  // namespace
-}  // namespace sg
-
 // A unit in 4 bits takes a third to two thirds of its bf16 time per key but as long for
 // what is fixed, and a long one holds the launch's end up as much: prefixes are cut so
 // that the estimated end of the last unit, and of the merge that pieces need, is earliest.
@@ -926,22 +923,14 @@ double end_of(std::vector<Alike>& units, int64_t slots) {
 // and 1 to 64 rows 436 us (693); 7 of 16,307-32,614 and one row 50 (63); 7 of 524-1,048
 // and 1 to 64 rows 22 (28); 64 of 512-4,096 and 16 to 128 rows 89 (89); d = 64, 2 of
 // 27,218 and 256 rows 163 (235).
-extern "C" int sg_tree_attn_plan_mx4(int32_t num_requests, const int32_t* row_offset_host,
-                                     const int32_t* prefix_len_host, int32_t num_q_heads,
-                                     int32_t num_kv_heads, int32_t head_dim, void* plan_host,
-                                     size_t plan_capacity_bytes, size_t* plan_bytes,
-                                     int32_t* plan_units, int32_t* plan_merges,
-                                     size_t* workspace_bytes) {
-  using namespace sg;
-  clear_error();
-  PlanWave wave = {num_requests, row_offset_host, prefix_len_host, num_q_heads, num_kv_heads,
-                   head_dim};
-  const PlanOut out = {plan_host,  plan_capacity_bytes, plan_bytes,
-                       plan_units, plan_merges,         workspace_bytes};
+int plan_mx4(PlanWave wave, const PlanOut& out) {
   if (const int rc = check_plan_wave(wave, out)) return rc;
-  const int G = num_q_heads / num_kv_heads;
+  const int num_requests = wave.num_requests, num_kv_heads = wave.num_kv_heads;
+  const int32_t* const row_offset_host = wave.row_offset;
+  const int32_t* const prefix_len_host = wave.prefix_len;
+  const int G = wave.num_q_heads / num_kv_heads;
   const int rpt = kQPerUnit / G;
-  const UnitCost& cost = head_dim == 64 ? kCost64 : kCost128;
+  const UnitCost& cost = wave.head_dim == 64 ? kCost64 : kCost128;
   // A unit of `rows` rows over `keys` keys, and over its request's tree if it is the
   // last piece.
   auto micros = [&](int rows, double keys, int tree_rows, bool alone) {
@@ -993,7 +982,7 @@ extern "C" int sg_tree_attn_plan_mx4(int32_t num_requests, const int32_t* row_of
       const int of = halves[i] ? rpt / 2 : rpt;
       count += static_cast<int64_t>((rows + of - 1) / of) * splits[i] * num_kv_heads;
       if (splits[i] > 1)
-        partial_bytes += 4.0 * (head_dim + 2) * rows * num_q_heads * splits[i];
+        partial_bytes += 4.0 * (wave.head_dim + 2) * rows * wave.num_q_heads * splits[i];
     }
     if (count > 8 * kSlots && cut.share > 0.0) continue;
     if (splits == last_splits && halves == last_halves) continue;
@@ -1047,6 +1036,24 @@ extern "C" int sg_tree_attn_plan_mx4(int32_t num_requests, const int32_t* row_of
     return static_cast<int64_t>(100.0 * micros(rows, 32.0 * tiles, 0, false));
   };
   return emit_plan(wave, out);
+}
+
+}  // namespace
+}  // namespace sg
+
+extern "C" int sg_tree_attn_plan_mx4(int32_t num_requests, const int32_t* row_offset_host,
+                                     const int32_t* prefix_len_host, int32_t num_q_heads,
+                                     int32_t num_kv_heads, int32_t head_dim, void* plan_host,
+                                     size_t plan_capacity_bytes, size_t* plan_bytes,
+                                     int32_t* plan_units, int32_t* plan_merges,
+                                     size_t* workspace_bytes) {
+  using namespace sg;
+  clear_error();
+  const PlanWave wave = {num_requests, row_offset_host, prefix_len_host,
+                         num_q_heads,  num_kv_heads,    head_dim};
+  const PlanOut out = {plan_host,  plan_capacity_bytes, plan_bytes,
+                       plan_units, plan_merges,         workspace_bytes};
+  return guarded([&] { return plan_mx4(wave, out); });
 }
 
 extern "C" int sg_tree_attn_mx4_fwd(const SgTreeAttnMx4Args* args, sg_stream_t stream) {
