@@ -9,10 +9,12 @@
 //
 // K is multiplied as it is held: v_mfma_scale_f32_32x32x64_f8f6f4 takes e2m1
 // elements with a power-of-two scale for 32 of them, so S^T = K Q^T needs no
-// unpacking and no LDS, if Q is in 8 bits.  A bf16 value's 8 significant bits are
-// the sum of two e4m3 values of 4 each, q = hi + lo exactly, with a scale for 32
-// columns (a value below 2^-14 of its block's largest keeps fewer bits, an error
-// below 2^-22 of that); two products each, in the time of the bf16 ones.
+// unpacking and no LDS, if Q is in 8 bits.  A bf16 value q is held as two e4m3 values
+// with scales for 32 columns: hi is q rounded to 4 significant bits, lo = q - hi has 4
+// at most and a scale 2^5 smaller; two products each, in the time of the bf16 ones.
+// q = hi + lo exactly from 2^-14 of its block's largest value on; below that hi is one
+// of e4m3's subnormals or 0 and lo is rounded to multiples of 2^-21 of a power of two
+// that the largest reaches, so the error is at most 2^-22 of the largest.
 // V is unpacked to bf16 (gfx950: two values an instruction, scale included) into
 // LDS and read transposed (ds_read_b64_tr_b16) for O^T += V^T P^T with
 // v_mfma_f32_32x32x16_bf16, as in tree_attn.hip.
@@ -536,32 +538,30 @@ __device__ __forceinline__ void attn_unit_mx4(const SgTreeAttnMx4Args& args, Arg
                                              w[e] & 0x7fff0000u);
       const auto both = __builtin_amdgcn_permlane32_swap(most, most, false, false);
       const int top = static_cast<int>(max(both[0], both[1]) >> 23);
-      code[b] = min(max(top - 7, 5), 254);  // the largest magnitude is below 256
+      code[b] = min(max(top - 7, 6), 254);  // the largest magnitude is in [128, 256)
       const float x_hi = __uint_as_float(static_cast<uint32_t>(code[b]) << 23);
-      const float x_lo = __uint_as_float(static_cast<uint32_t>(code[b] - 4) << 23);
+      const float x_lo = __uint_as_float(static_cast<uint32_t>(code[b] - 5) << 23);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         short2_t hi = {0, 0}, lo = {0, 0};
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const uint32_t whole = w[2 * e + k], head4 = whole & 0xfff0fff0u;
-          const float lo0 = __uint_as_float(whole << 16) - __uint_as_float(head4 << 16);
-          const float lo1 =
-              __uint_as_float(whole & 0xffff0000u) - __uint_as_float(head4 & 0xffff0000u);
-          if (k == 0) {
-            hi = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(hi, as_pair(head4), x_hi, false);
-            lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(lo, lo0, lo1, x_lo, false);
-          } else {
-            hi = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(hi, as_pair(head4), x_hi, true);
-            lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(lo, lo0, lo1, x_lo, true);
-          }
-        }
+        // lo is what hi's codes leave of q, whichever way they were rounded.
+        auto pair = [&](uint32_t whole, auto upper) {
+          constexpr bool kUpper = decltype(upper)::value;
+          hi = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(hi, as_pair(whole), x_hi, kUpper);
+          const auto held = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(
+              __builtin_bit_cast(uint32_t, hi), x_hi, kUpper);
+          lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(
+              lo, __uint_as_float(whole << 16) - held[0],
+              __uint_as_float(whole & 0xffff0000u) - held[1], x_lo, kUpper);
+        };
+        pair(w[2 * e], std::false_type{});
+        pair(w[2 * e + 1], std::true_type{});
         // An infinity or a NaN: the block is NaN.
         q_hi[j][4 * b + e] = top == 255 ? 0x7f7f7f7f : __builtin_bit_cast(int, hi);
         q_lo[j][4 * b + e] = __builtin_bit_cast(int, lo);
       }
     }
-    q_scale[j] = half == 0 ? code[0] | (code[0] - 4) << 8 : code[1] | (code[1] - 4) << 8;
+    q_scale[j] = half == 0 ? code[0] | (code[0] - 5) << 8 : code[1] | (code[1] - 5) << 8;
   }
 
   auto qk = [&](const Raw& r) {

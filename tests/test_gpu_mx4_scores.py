@@ -1,0 +1,84 @@
+"""Scores of the attention over a 4-bit cache where they are hardest: outlier columns,
+large scores, wide ranges inside a block of 32 columns, and values that are no numbers.
+
+Tolerance, before any run.  Three things put a score s = scale * sum_c k_c q_c off.
+q is held as two e4m3 values: exactly from 2^-14 of its block's largest value on, else
+within 2^-22 of that.  The matrix instruction adds 8 products on the exponent of the
+largest of them and drops what lies 2^-14 below it, so 8 products are off by at most 7 * 2^-14
+of their largest and a sum of them by less than 2^-11 of sum |k q| for each of the two
+terms (the second one's products are 2^-4 of the first one's).  fp32 sums of the parts:
+2^-20 of sum |k q| at most.  With a score off by at most D everywhere a probability is
+off by a factor within exp(+-2 D), so an output by (exp(2 D) - 1) sum(p |v|), beside
+what the attention's other tests allow.
+"""
+import pytest
+import torch
+
+from tests import mx4_cases as M
+from tests.test_gpu_mx4_attention import Wave
+
+pytestmark = pytest.mark.gpu
+
+
+def _set_k(w, change):
+    """Repack the prefix's K after change(values [Hkv, tokens, D])."""
+    behind = w.scales[0].cpu() == 255
+    k = torch.nan_to_num(M.values(w.codes[0], w.scales[0]))
+    k = change(k).to(torch.bfloat16)
+    codes, scales = M.pack(k)
+    scales[behind] = 255
+    w.codes[0], w.scales[0] = codes.to(w.device), scales.to(w.device)
+
+
+def _worst(w, out):
+    """The largest error against its bound, and the largest D."""
+    worst, most = 0.0, 0.0
+    for i in range(len(w.lengths)):
+        a, b = int(w.offset[i]), int(w.offset[i + 1])
+        want, bound = w.reference(i)
+        at = slice(int(w.start[i]), int(w.start[i]) + int(w.lengths[i]))
+        k = torch.cat([M.values(w.codes[0][:, at], w.scales[0][:, at]),
+                       w.tree[0][a:b].double().cpu().transpose(0, 1)], 1)
+        v = torch.cat([M.values(w.codes[1][:, at], w.scales[1][:, at]),
+                       w.tree[1][a:b].double().cpu().transpose(0, 1)], 1)
+        group = w.hq // w.hkv
+        k, v = k.repeat_interleave(group, 0), v.repeat_interleave(group, 0)
+        q = w.q[a:b].double().cpu().transpose(0, 1)
+        blocks = q.abs().unflatten(2, (-1, 32))
+        most_q = blocks.amax(3, keepdim=True)
+        lost = torch.where(blocks < 2.0 ** -14 * most_q, 2.0 ** -22 * most_q, 0.0).flatten(2)
+        off = ((2.0 ** -11 * (1 + 2.0 ** -4) + 2.0 ** -20) * (q.abs() @ k.abs().transpose(1, 2))
+               + lost @ k.abs().transpose(1, 2)) * w.dim ** -0.5
+        d = off.amax(2).transpose(0, 1)[..., None]
+        # sum(p |v|) again, from the bound: it is (bound - 2^-8 |out|) / (2^-8 + 2^-12).
+        mass = (bound - 2.0 ** -8 * want.abs()) / (2.0 ** -8 + 2.0 ** -12)
+        bound = bound + torch.expm1(2 * d) * mass
+        err = (out[a:b].double().cpu() - want).abs()
+        assert torch.isfinite(out[a:b]).all()
+        worst = max(worst, float((err / bound).max()))
+        most = max(most, float(d.max()))
+    return worst, most
+
+
+@pytest.mark.parametrize("ratio", [10, 13, 14, 17, 20])
+@pytest.mark.parametrize("dim,rows", [(64, [3, 40]), (128, [1, 7]), (128, [16, 33])])
+def test_one_large_q_channel_that_meets_no_key(device, ratio, dim, rows):
+    """Every block of q has a channel 2^ratio times the others' least magnitude; all
+    keys are 0 there, so the scores are the other channels' alone."""
+    w = Wave(device, [300, 129], rows, 8, 2, dim, seed=ratio + dim)
+    lone = torch.arange(5, dim, 32)
+    g = torch.Generator().manual_seed(ratio)
+    q = (1 + torch.rand(w.q.shape, generator=g)) * torch.randn(w.q.shape, generator=g).sign()
+    q = q.to(torch.bfloat16)
+    q[..., lone] = 2.0 ** ratio
+    w.q = q.to(device)
+
+    def clear(k):
+        k[..., lone] = 0
+        return k
+
+    _set_k(w, clear)
+    w.tree[0][..., lone.to(device)] = 0
+    worst, most = _worst(w, w.run())
+    assert worst <= 1.0
+    assert ratio > 14 or most < 0.02  # the bound itself says something
