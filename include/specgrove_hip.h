@@ -513,7 +513,11 @@ int sg_tree_attn_plan_mx4(int32_t num_requests, const int32_t* row_offset_host,
                           size_t plan_capacity_bytes, size_t* plan_bytes, int32_t* plan_units,
                           int32_t* plan_merges, size_t* workspace_bytes);
 
-/* sg_tree_attn_fwd over a 4-bit prefix (the wave's own rows are bf16). */
+/* sg_tree_attn_fwd over a 4-bit prefix (the wave's own rows are bf16).  Scores of the
+ * prefix are narrower than sg_tree_attn_fwd's: q is exact from 2^-14 of the largest
+ * value of its 32 columns on, else within 2^-22 of that, and the sum of a key's
+ * products is off by less than 2^-11 of the sum of their magnitudes (2^-20 in the mean
+ * over Gaussian rows).  A query vector with an infinity or a NaN gives NaN. */
 typedef struct SgTreeAttnMx4Args {
   SgTreeAttnArgs attn;        /* k/v_cache_dev: codes, 16-byte aligned; the cache strides are
                                  in bytes, multiples of 16 */
@@ -566,7 +570,9 @@ int sg_fp8_pack_weight(const void* weight_dev, int64_t weight_row_stride, int32_
 
 /* out[r, c] = bf16(sum over 128-column blocks b of
  *   row_scale[b, r] * weight_scale[c/128, b] * sum_k code[r, k] * weight[c, k]).
- * Sums are fp32; a block's products are added by the matrix instruction. */
+ * Sums are fp32, but a block's products are added by the matrix instruction, 8 at a
+ * time on the exponent of the largest: a block's sum is off by less than 2^-11 of the
+ * sum of their magnitudes. */
 typedef struct SgFp8MatmulArgs {
   int32_t num_rows;                /* R */
   int32_t n;                       /* output columns */

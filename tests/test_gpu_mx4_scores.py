@@ -82,3 +82,51 @@ def test_one_large_q_channel_that_meets_no_key(device, ratio, dim, rows):
     worst, most = _worst(w, w.run())
     assert worst <= 1.0
     assert ratio > 14 or most < 0.02  # the bound itself says something
+
+
+@pytest.mark.parametrize("dim,rows", [(64, [5, 40]), (128, [1, 16]), (128, [33, 64])])
+@pytest.mark.parametrize("kind", ["keys", "queries", "both", "large", "wide"])
+def test_outliers_and_large_scores(device, kind, dim, rows):
+    w = Wave(device, [700, 95], rows, 8, 2, dim, seed=dim + len(kind))
+    lone = torch.tensor([3, 40])
+    g = torch.Generator().manual_seed(7)
+    if kind in ("keys", "both"):        # a few columns far larger, as keys have them
+        def grow(k):
+            k[..., lone] *= 30
+            return k
+        _set_k(w, grow)
+    if kind in ("queries", "both"):
+        w.q[..., lone.to(device)] *= 20.0 if kind == "queries" else 4.0
+    if kind == "large":                 # scores of some tens
+        w.q *= 8.0
+    if kind == "wide":                  # 2^-16 to 1 of the block's largest, everywhere
+        w.q *= torch.exp2(torch.randint(-16, 1, w.q.shape, generator=g)).to(w.q)
+        _set_k(w, lambda k: k * torch.exp2(torch.randint(-6, 1, k.shape, generator=g)))
+    worst, _ = _worst(w, w.run())
+    assert worst <= 1.0
+
+
+@pytest.mark.parametrize("rows", [[1, 3], [16, 3], [33, 3]])
+def test_a_cached_key_that_is_no_number_reaches_its_heads_rows(device, rows):
+    w = Wave(device, [70, 40], rows, 8, 2, 128, seed=3)
+    clean = w.run()
+    w.scales[0][1, 11, 2] = 255          # K of token 11 of request 0, kv head 1
+    got = w.run()
+    assert torch.isnan(got[:rows[0], 4:]).all()
+    keep = torch.ones_like(got, dtype=torch.bool)
+    keep[:rows[0], 4:] = False
+    assert torch.equal(got[keep], clean[keep])
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+@pytest.mark.parametrize("rows", [[4, 3], [16, 3], [33, 3]])
+def test_a_query_that_is_no_number_gives_its_own_vector(device, rows, bad):
+    w = Wave(device, [70, 40], rows, 8, 2, 128, seed=4)
+    clean, bound = (torch.cat(t) for t in zip(*(w.reference(i) for i in range(2))))
+    w.q[2, 5, 77] = bad
+    got = w.run()
+    assert torch.isnan(got[2, 5]).all()
+    keep = torch.ones(got.shape, dtype=torch.bool)
+    keep[2, 5] = False
+    err = (got.double().cpu() - clean).abs()
+    assert bool((err <= bound)[keep].all())
