@@ -186,7 +186,7 @@ EXPORTED_SYMBOLS = (
     "sg_tree_attn_plan_mx4",
     "sg_fp8_quantize_rows", "sg_add_rmsnorm_fp8", "sg_silu_mul_fp8",
     "sg_fp8_packed_bytes", "sg_fp8_pack_weight", "sg_fp8_matmul",
-    "sg_fp8_matmul_workspace_bytes",
+    "sg_fp8_matmul_workspace_bytes", "sg_fp8_matmul_form",
 )
 
 # Static scratch of sg_tree_sample_noalloc (SG_TREE_SAMPLE_NOALLOC_SCRATCH_BYTES).
@@ -287,6 +287,8 @@ def load() -> ctypes.CDLL:
     lib.sg_fp8_pack_weight.argtypes = [c_void_p, c_i64, c_i32, c_i32, c_void_p, c_void_p]
     lib.sg_fp8_matmul_workspace_bytes.restype = c_i64
     lib.sg_fp8_matmul_workspace_bytes.argtypes = [c_i32, c_i32, c_i32]
+    lib.sg_fp8_matmul_form.restype = c_i32
+    lib.sg_fp8_matmul_form.argtypes = [c_i32, c_i32, c_i32]
     lib.sg_fp8_matmul.restype = c_i32
     lib.sg_fp8_matmul.argtypes = [ctypes.POINTER(SgFp8MatmulArgs), c_void_p]
     lib.sg_clock_probe.restype = c_i32
