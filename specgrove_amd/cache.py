@@ -86,11 +86,11 @@ class PersistentRequestCacheLayer:
 
     @property
     def keys(self) -> torch.Tensor:
-        return self._cache.pool._cached_rows(self._layer_index, *self._span())[0].unsqueeze(0)
+        return self._cache.pool._cached_rows(0, self._layer_index, *self._span()).unsqueeze(0)
 
     @property
     def values(self) -> torch.Tensor:
-        return self._cache.pool._cached_rows(self._layer_index, *self._span())[1].unsqueeze(0)
+        return self._cache.pool._cached_rows(1, self._layer_index, *self._span()).unsqueeze(0)
 
 
 class PersistentRequestCache:
@@ -130,23 +130,25 @@ class PersistentRequestCachePool:
         layers = len(caches[0].layers)
         if any(len(cache.layers) != layers for cache in caches):
             raise ValueError("Target caches have different layer counts")
-        first = caches[0].layers
-        if any(layer.keys.shape[0] != 1 for cache in caches for layer in cache.layers):
+        # (A layer of a pool holds one request; a 4-bit one would unpack its rows here.)
+        if any(layer.keys.shape[0] != 1 for cache in caches for layer in cache.layers
+               if not isinstance(layer, PersistentRequestCacheLayer)):
             raise ValueError("Expected one request per source cache")
+        first = caches[0].layers[0].keys
         self.capacity = int(capacity)
         self.lengths = list(lengths)
         self.num_layers = layers
-        self.device = first[0].keys.device
+        self.device = first.device
         self._k_ptrs = None
         self._v_ptrs = None
         self._commit = None          # prepared commit call and its metadata buffers
         self._status = None          # DeviceStatus of the commits, made by the first one
-        self._fill(caches)
+        self._fill(caches, first)
         self.caches = tuple(PersistentRequestCache(self, slot) for slot in range(len(caches)))
 
-    def _fill(self, caches: Sequence) -> None:
-        """Allocate the arena and copy the requests' prefills in."""
-        first = caches[0].layers[0].keys
+    def _fill(self, caches: Sequence, first: torch.Tensor) -> None:
+        """Allocate the arena and copy the requests' prefills in; first: the first
+        one's keys of layer 0."""
         hkv, dim = first.shape[1], first.shape[-1]
         arena = torch.empty((2, self.num_layers, hkv, len(caches) * self.capacity, dim),
                             dtype=first.dtype, device=first.device)
@@ -160,9 +162,9 @@ class PersistentRequestCachePool:
         self.key_storage: list[torch.Tensor] = list(arena[0].unbind(0))
         self.value_storage: list[torch.Tensor] = list(arena[1].unbind(0))
 
-    def _cached_rows(self, layer: int, start: int, end: int):
-        """K and V [Hkv, end - start, D] of the arena's rows."""
-        return self.key_storage[layer][:, start:end], self.value_storage[layer][:, start:end]
+    def _cached_rows(self, which: int, layer: int, start: int, end: int) -> torch.Tensor:
+        """K (which = 0) or V [Hkv, end - start, D] of the arena's rows."""
+        return (self.key_storage, self.value_storage)[which][layer][:, start:end]
 
     @property
     def status(self) -> DeviceStatus:
@@ -318,18 +320,19 @@ class Mx4RequestCachePool(PersistentRequestCachePool):
     rows unpacked into a new bf16 tensor, what the attention multiplies.
     """
 
-    def _fill(self, caches: Sequence) -> None:
-        first = caches[0].layers[0].keys
+    def _fill(self, caches: Sequence, first: torch.Tensor) -> None:
         hkv, dim = first.shape[1], first.shape[-1]
         if dim not in (64, 128):
             raise ValueError("A 4-bit cache needs head_dim 64 or 128")
-        for cache, length in zip(caches, self.lengths):
-            for layer in cache.layers:
-                for t in (layer.keys, layer.values):
-                    if t.dtype != torch.bfloat16 or t.device != first.device:
-                        raise ValueError("A 4-bit cache takes bf16 caches of one device")
-                    if t.shape != (1, hkv, length, dim):
-                        raise ValueError("Expected keys and values [1, Hkv, L, D]")
+        # Read once: what a layer gives may be made at the read (rows of another pool).
+        rows = [[layer.keys for layer in cache.layers] + [layer.values for layer in cache.layers]
+                for cache in caches]
+        for tensors, length in zip(rows, self.lengths):
+            for t in tensors:
+                if t.dtype != torch.bfloat16 or t.device != first.device:
+                    raise ValueError("A 4-bit cache takes bf16 caches of one device")
+                if t.shape != (1, hkv, length, dim):
+                    raise ValueError("Expected keys and values [1, Hkv, L, D]")
         if first.device.type != "cuda":
             raise ValueError("A 4-bit cache lives on the GPU")
         slots = len(caches)
@@ -346,7 +349,7 @@ class Mx4RequestCachePool(PersistentRequestCachePool):
         filled = [slot for slot in range(slots) if self.lengths[slot] > 0]
         if not filled:
             return
-        sources = [self._tree_rows(caches[slot]) for slot in filled]
+        sources = [self._tree_rows(rows[slot]) for slot in filled]
         words = np.zeros((len(filled), 3 + 2 * self.num_layers), np.int64)
         for row, slot, tensors in zip(words, filled, sources):
             row[0] = slot * self.capacity
@@ -364,19 +367,19 @@ class Mx4RequestCachePool(PersistentRequestCachePool):
                                             tree_head_stride=k0.stride(1))()
         self.status.after_launch()
 
-    def _tree_rows(self, cache) -> list[torch.Tensor]:
-        """K of every layer, then V, as [L, Hkv, D] views of one layout."""
-        tensors = [layer.keys[0] for layer in cache.layers]
-        tensors += [layer.values[0] for layer in cache.layers]
+    def _tree_rows(self, tensors: Sequence[torch.Tensor]) -> list[torch.Tensor]:
+        """K of every layer, then V, [1, Hkv, L, D], as [L, Hkv, D] views of one layout."""
+        tensors = [t[0] for t in tensors]
         s = tensors[0].stride()
         if s[2] != 1 or (s[0] | s[1]) % 8 or any(
                 t.stride() != s or t.data_ptr() % 16 for t in tensors):
             tensors = [t.clone(memory_format=torch.contiguous_format) for t in tensors]
         return [t.transpose(0, 1) for t in tensors]
 
-    def _cached_rows(self, layer: int, start: int, end: int):
-        return tuple(ops.kv_load_mx4(c[layer][:, start:end], s[layer][:, start:end])
-                     for c, s in ((self.k_codes, self.k_scales), (self.v_codes, self.v_scales)))
+    def _cached_rows(self, which: int, layer: int, start: int, end: int) -> torch.Tensor:
+        codes, scales = ((self.k_codes, self.k_scales), (self.v_codes, self.v_scales))[which]
+        with torch.cuda.device(self.device):  # whichever device is current, as a bf16 pool's
+            return ops.kv_load_mx4(codes[layer][:, start:end], scales[layer][:, start:end])
 
     def _device_pointers(self):
         if self._k_ptrs is None:
