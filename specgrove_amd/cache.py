@@ -356,15 +356,18 @@ class Mx4RequestCachePool(PersistentRequestCachePool):
             row[1:3].view(np.int32)[:] = [0, self.lengths[slot], self.lengths[slot], 0]
             row[3:] = [t.data_ptr() for t in tensors]
         meta = ops.upload(words.reshape(-1), first.device).view(len(filled), -1)
-        for row, tensors in zip(meta, sources):
+        for row, slot, tensors in zip(meta, filled, sources):
             counts = row[1:3].view(torch.int32)
             k0 = tensors[0]
+            # (The prompt's rows and not the slot's: 500 tokens in a slot of 32,768
+            # would start 64 workgroups for each that has work.)
             self._prepare_commit(
                 self.num_layers, row[3:3 + self.num_layers], row[3 + self.num_layers:],
                 row_offset=counts[:2], keep_rows=None, keep_len=counts[2:3],
                 prefix_start=row[:1], lengths=counts[3:4], capacity=self.capacity,
                 status=self.status.dev).set(tree_row_stride=k0.stride(0),
-                                            tree_head_stride=k0.stride(1))()
+                                            tree_head_stride=k0.stride(1),
+                                            keep_stride=self.lengths[slot])()
         self.status.after_launch()
 
     def _tree_rows(self, tensors: Sequence[torch.Tensor]) -> list[torch.Tensor]:

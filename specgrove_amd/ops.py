@@ -1079,7 +1079,9 @@ def prepare_kv_commit_mx4(k_code_ptrs: torch.Tensor, k_scale_ptrs: torch.Tensor,
 
     ``*_ptrs`` are int64 device arrays of per-layer base addresses; the strides of
     codes and scales are in bytes.  ``keep_rows`` [n, keep_stride] i32, or None: a
-    request keeps its rows 0 .. keep_len - 1 (a prefilled prompt).
+    request keeps its rows 0 .. keep_len - 1 (a prefilled prompt).  The launch then covers
+    ``capacity`` rows a request; ``set(keep_stride=...)`` of the prepared call bounds it
+    by the longest prompt, where the host knows that (a longer one reports SG_ERANGE).
     """
     pointers = (k_code_ptrs, k_scale_ptrs, v_code_ptrs, v_scale_ptrs, k_tree_ptrs, v_tree_ptrs)
     names = ("k_code_ptrs", "k_scale_ptrs", "v_code_ptrs", "v_scale_ptrs", "k_tree_ptrs",
