@@ -682,9 +682,14 @@ struct Cut {
   int splits;
 };
 
-// Rows up to 32 (up to 64 where the second pair of row blocks finds the weight in
-// L2, N <= 12,288) take the few-rows kernel: 64 rows of 4096 -> 4096 in 7.5 us, a
-// tile kernel 11.6; of 4096 -> 24576 in 31, a tile kernel 18.8.  Two weight blocks a
+// Rows up to 32 take the few-rows kernel; 33 to 64, which read the weight twice there,
+// while it has at most 48 MiB (N x K).  Few-rows and tile kernels at 64 rows, a launch's
+// share of many with weights from HBM: 2560 -> 6144 in 9.8 and 13.6 us, 4096 -> 4096 9.0
+// and 15.3, 4096 -> 12288 20.8 and 18.9, 12288 -> 4096 19.5 and 19.0; 12288 -> 6144 34.7
+// and 26.9, 4096 -> 16384 26.4 and 21.2, 4096 -> 24576 38.6 and 24.6 (33 rows: 8.2 and
+// 11.5, 8.4 and 13.2, 18.7 and 18.9, 17.9 and 17.8; 28.2 and 24.5, 24.8 and 20.1, 36.3
+// and 22.7).  Whether a weight block's two readers share an XCD makes no difference
+// (4096 -> 6144, where they do, 14.0; 6176, where they do not, 14.1).  Two weight blocks a
 // wave once that leaves 160 workgroups (6144 x 2560 at 16 rows 4.4 us, one block 5.2;
 // at 32 rows 7.7 and 9.4; 4096 x 12288 the other way round, 10.8 and 9.4, at 32 rows
 // 21.2 and 18.5).
@@ -701,7 +706,8 @@ struct Cut {
 // pairs 20.
 Cut cut_of(int rows, int n, int steps) {
   if (rows <= 16) return {n > 32 * 159 ? kFew2 : kFew1, 1};
-  if (rows <= 32 || (rows <= 64 && n <= 12288))
+  const int64_t weight_bytes = static_cast<int64_t>(n) * steps * kBlockK;
+  if (rows <= 32 || (rows <= 64 && weight_bytes <= (48 << 20)))
     return {(n + 31) / 32 * ((rows + 31) / 32) < 160 ? kFew1x2 : kFew2x2, 1};
   struct Kind {
     Form form;

@@ -33,3 +33,14 @@ def test_sizes_without_a_form():
     assert lib.sg_fp8_matmul_form(-1, 256, 256) == -1
     assert lib.sg_fp8_matmul_form(4, 0, 256) == -1
     assert lib.sg_fp8_matmul_form(4, 256, (1 << 24) + 1) == -1
+
+
+def test_a_large_weight_is_not_read_twice():
+    """33 to 64 rows: the few-rows kernel (forms 0 to 3) up to 48 MiB of weight, whichever
+    way the weight is long."""
+    for rows in (33, 64):
+        for k, n in ((2560, 6144), (4096, 12288), (12288, 4096), (4100, 11900)):
+            assert _form(rows, k, n)[0] < 4
+        for k, n in ((12288, 6144), (12288, 12288), (4096, 16384), (4096, 12289), (12289, 4096)):
+            assert _form(rows, k, n)[0] >= 4
+    assert _form(32, 12288, 12288)[0] < 4
