@@ -256,7 +256,7 @@ def _prepare_attn(c, g):
                  _dev(np.concatenate(parents).astype(np.int32)))
     if own:
         from specgrove_amd import ops
-        s["plan"] = ops.plan_attention(offset, lengths, c["hq"], c["hkv"], d).to(DEVICE)
+        s["plan"] = ops.plan_attention_mx4(offset, lengths, c["hq"], c["hkv"], d).to(DEVICE)
     return s
 
 
