@@ -42,15 +42,15 @@
 // workgroups share a CU; streams are merged at the end.
 //
 // Measured (64 requests of 16,384 cached tokens, 32 q / 8 kv heads, d = 128; 1 / 16 /
-// 32 rows each): 234 / 365 / 619 us, that is 4.9 / 3.1 / 1.8 TB/s of codes and scales
-// and 73 / 753 / 888 TFLOP/s.  One row a request is bound by the cache's bytes, 32
-// by issue: a wave and tile take 124 vector instructions and 12 products, of which a
+// 32 rows each): 240 / 363 / 597 us, that is 4.8 / 3.1 / 1.9 TB/s of codes and scales
+// and 72 / 757 / 921 TFLOP/s.  One row a request is bound by the cache's bytes, 32
+// by issue: a wave and tile take 119 vector instructions and 12 products, of which a
 // wave alone on its SIMD can overlap little (450 us for half the requests, one workgroup
-// a CU).  Tried: K and V unpacked to bf16 by the workgroup, 406 / 444 / 702; by each wave
-// for itself, 249 / 470 / 873; the products of a tile issued before the softmax of the
-// one before it, 583 / 381 / 672 (spills at one row); all of V read before the softmax,
-// 314 / 369 / 620; K two tiles ahead for 3-4 q-groups too (spills), 243 / 433 / 664;
-// s_setprio around the products, no difference.
+// a CU).  Tried, at 234 / 365 / 619 us: K and V unpacked to bf16 by the workgroup, 406 /
+// 444 / 702; by each wave for itself, 249 / 470 / 873; the products of a tile issued
+// before the softmax of the one before it, 583 / 381 / 672 (spills at one row); all of V
+// read before the softmax, 314 / 369 / 620; K two tiles ahead for 3-4 q-groups too
+// (spills), 243 / 433 / 664; s_setprio around the products, no difference.
 #include <algorithm>
 #include <cmath>
 #include <map>
@@ -933,10 +933,10 @@ double end_of(std::vector<Alike>& units, int64_t slots) {
 // A unit in 4 bits takes a third to two thirds of its bf16 time per key but as long for
 // what is fixed, and a long one holds the launch's end up as much: prefixes are cut so
 // that the estimated end of the last unit, and of the merge that pieces need, is earliest.
-// Against the bf16 plan, 32 q / 8 kv heads, d = 128: 32 requests of 8,192-32,768 tokens
-// and 1 to 64 rows 436 us (693); 7 of 16,307-32,614 and one row 50 (63); 7 of 524-1,048
-// and 1 to 64 rows 22 (28); 64 of 512-4,096 and 16 to 128 rows 89 (89); d = 64, 2 of
-// 27,218 and 256 rows 163 (235).
+// Against the bf16 plan, in turn, 32 q / 8 kv heads, d = 128: 32 requests of 8,192-32,768
+// tokens and 1 to 64 rows 432 us (692); 7 of 16,307-32,614 and one row 48 (65); 7 of
+// 524-1,048 and 1 to 64 rows 25 (29); 64 of 512-4,096 and 16 to 128 rows 84 (85); d = 64,
+// 2 of 27,218 and 256 rows 162 (234).
 int plan_mx4(PlanWave wave, const PlanOut& out) {
   if (const int rc = check_plan_wave(wave, out)) return rc;
   const int num_requests = wave.num_requests, num_kv_heads = wave.num_kv_heads;
