@@ -517,7 +517,8 @@ int sg_tree_attn_plan_mx4(int32_t num_requests, const int32_t* row_offset_host,
  * prefix are narrower than sg_tree_attn_fwd's: q is exact from 2^-14 of the largest
  * value of its 32 columns on, else within 2^-22 of that, and the sum of a key's
  * products is off by less than 2^-10 of the sum of their magnitudes (2^-20 in the mean
- * over Gaussian rows).  A query vector with an infinity or a NaN gives NaN. */
+ * over Gaussian rows).  A query vector with an infinity or a NaN gives NaN.
+ * scale must be positive and finite. */
 typedef struct SgTreeAttnMx4Args {
   SgTreeAttnArgs attn;        /* k/v_cache_dev: codes, 16-byte aligned; the cache strides are
                                  in bytes, multiples of 16 */

@@ -1077,6 +1077,8 @@ extern "C" int sg_tree_attn_mx4_fwd(const SgTreeAttnMx4Args* args, sg_stream_t s
   const SgTreeAttnArgs& a = args->attn;
   AttnCall call;
   if (const int rc = check_attn_call(a, &call)) return rc;
+  // The running maximum is one of raw scores.
+  SG_REQUIRE(a.scale > 0.0f && std::isfinite(a.scale), "scale must be positive and finite");
   if (a.plan_units == 0) return SG_OK;
   SG_REQUIRE(args->k_scale_dev && args->v_scale_dev, "null device pointer");
   SG_REQUIRE(a.cache_head_stride % 16 == 0 && a.cache_token_stride % 16 == 0 &&

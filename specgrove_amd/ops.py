@@ -929,7 +929,8 @@ def prepare_tree_attention_mx4(q: torch.Tensor, k_codes: torch.Tensor, k_scales:
     layer's arena, rows written by ``kv_commit_mx4``); everything else, the plan
     included, as in ``prepare_tree_attention``.  What lies behind a request's
     last token is not looked at.  An infinity or a NaN in a tree row reaches only
-    the rows that see it; a cached row packed from one gives NaN.
+    the rows that see it; a cached row packed from one gives NaN.  ``scale`` (positive,
+    finite; head_dim ** -0.5 without it) is checked by the call itself.
     """
     args, out, run = _mx4_attention_args(q, k_codes, k_scales, v_codes, v_scales, k_tree, v_tree,
                                          row_offset, prefix_start, prefix_len, parent, plan, out,

@@ -10,7 +10,7 @@ import numpy as np
 import pytest
 import torch
 
-from specgrove_amd import ops
+from specgrove_amd import _lib, ops
 
 WAVE = ([0, 1, 2], [32768, 300])
 
@@ -139,3 +139,19 @@ def test_arguments_that_fit_are_looked_at_once(monkeypatch):
                 dict(status=status.long()), dict(out=[1]), dict(status=1)):
         with pytest.raises(ValueError):
             _call(plan, **bad)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.1, float("inf"), float("nan")])
+def test_scales_that_are_no_scales_are_refused(scale):
+    """(An empty wave: nothing would be launched.)"""
+    plan = ops.plan_attention_mx4([0], [], 8, 2, 64).to("cpu")
+    q, tree = torch.zeros((0, 8, 64)), torch.zeros((0, 2, 64))
+    q, tree = q.to(torch.bfloat16), tree.to(torch.bfloat16)
+    codes = torch.zeros((2, 16, 32), dtype=torch.uint8)
+    scales = torch.zeros((2, 16, 2), dtype=torch.uint8)
+    meta = _meta_tensors([0], [])
+    for value, code in ((scale, -1), (0.125, 0)):
+        call = ops.prepare_tree_attention_mx4(q, codes, scales, codes, scales, tree, tree, *meta,
+                                              plan, scale=value)
+        assert _lib.load().sg_tree_attn_mx4_fwd(call._ref, None) == code
+        assert call.result.shape == (0, 8, 64)
